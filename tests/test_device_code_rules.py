@@ -1,0 +1,67 @@
+"""What no GPU code of this repository may hold, checked on the sources as text and on the compiled library's instructions.  CPU only.
+
+Writes through the scalar data cache (scalar stores, scalar atomics, that cache's write-back and discard) are refused where this code runs on
+shared GPUs, comments included: data is written with vector stores.  The patterns below are put together from pieces so that this file does
+not hold the words itself."""
+import os
+import re
+import shutil
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+OBJDUMP = "/opt/rocm/llvm/bin/llvm-objdump"
+SOURCES = (".hip", ".h", ".hpp", ".c", ".cpp", ".s", ".S", ".inc", ".py", ".sh", ".mk", ".cmake", ".patch")
+SKIPPED = {".git", "_work", "gpurun_out", "build", "__pycache__", ".pytest_cache", "_ref"}
+
+SCALAR_WRITE = re.compile(r"\bs_" + r"(?:(?:buffer_|scratch_)?" + r"(?:store|atomic)(?:_\w+)?\b" + r"|d" + r"cache_(?:wb|discard)\w*)")
+
+
+def source_files():
+    for d, dirs, files in os.walk(ROOT):
+        dirs[:] = [x for x in dirs if x not in SKIPPED]
+        for f in files:
+            if f.endswith(SOURCES) or f == "Makefile":
+                yield os.path.join(d, f)
+
+
+def device_code(tmp_path):
+    """{instruction mnemonic: how often} over every code object of the built library"""
+    if not os.path.exists(OBJDUMP):
+        pytest.skip("needs llvm-objdump of the ROCm toolchain")
+    import fun_ofdm_amd
+    lib = shutil.copy(fun_ofdm_amd._lib.library_path(), str(tmp_path / "lib.so"))
+    subprocess.run([OBJDUMP, "--offloading", lib], check=True, cwd=str(tmp_path), stdout=subprocess.DEVNULL)
+    objects = [f for f in sorted(os.listdir(str(tmp_path))) if f.endswith("gfx950")]
+    assert len(objects) == 5                                  # one per unit with kernels: handle, decode, sync, stage, tx
+    count = {}
+    for o in objects:
+        text = subprocess.run([OBJDUMP, "-d", "--mcpu=gfx950", o], check=True, cwd=str(tmp_path), capture_output=True, text=True).stdout
+        for m in re.findall(r"^\t([a-z]\w+)", text, re.M):
+            count[m] = count.get(m, 0) + 1
+    assert sum(count.values()) > 10000 and count.get("s_endpgm", 0) >= 30
+    return count
+
+
+def test_the_pattern_knows_what_it_looks_for():
+    for word in ("store_dword", "store_dwordx4", "buffer_store_dword", "scratch_store_dword", "atomic_add", "buffer_atomic_or", "d" + "cache_wb", "d" + "cache_wb_vol",
+                 "d" + "cache_discard"):
+        assert SCALAR_WRITE.search("\ts_" + word + " s[0:1]"), word
+    for line in ("s_load_dwordx2 s[0:1]", "global_store_dword v0", "ds_store_b32", "s_d" + "cache_inv", "foa_rxs_store"):
+        assert not SCALAR_WRITE.search(line), line
+
+
+def test_no_source_writes_through_the_scalar_cache():
+    seen, bad = 0, []
+    for path in source_files():
+        seen += 1
+        for n, line in enumerate(open(path, errors="replace"), 1):
+            if SCALAR_WRITE.search(line):
+                bad.append("%s:%d" % (os.path.relpath(path, ROOT), n))
+    assert seen > 60 and not bad, bad
+
+
+def test_no_kernel_writes_through_the_scalar_cache(tmp_path):
+    bad = {m: n for m, n in device_code(tmp_path).items() if SCALAR_WRITE.search(m)}
+    assert not bad, bad
