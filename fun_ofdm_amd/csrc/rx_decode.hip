@@ -171,6 +171,7 @@ int foa_rx_decode_frames_ctx_dev(foa_rx *rx, const float *d_iq, size_t n_samples
 int foa_rx_decode_frames_lead_ctx_dev(foa_rx *rx, const float *d_iq, size_t n_samples, const foa_frame_desc *d_descs, const int64_t *d_ends,
                                       size_t n_lead, size_t n_frames, size_t n_context, uint8_t *d_psdu, size_t slot_bytes, foa_frame_result *d_results)
 {
+    AfterScope taken(rx);
     if (n_lead > 0x7FFFFFF0u) return fail(FOA_E_INVALID, "too many frames");
     if ((n_lead || n_frames) && (!d_descs || !d_ends)) return fail(FOA_E_INVALID, "NULL device pointer");
     return decode_frames_any(rx, d_iq, false, n_samples, d_descs + n_lead, d_ends + n_lead, n_frames, n_context, n_lead, d_psdu, slot_bytes, d_results);
@@ -182,8 +183,9 @@ int foa_rx_decode_frames_lead_ctx_dev(foa_rx *rx, const float *d_iq, size_t n_sa
 static int decode_frames_any(foa_rx *rx, const void *d_iq, bool f64, size_t n_samples, const foa_frame_desc *d_descs, const int64_t *d_ends,
                              size_t n_frames, size_t n_context, size_t n_lead, uint8_t *d_psdu, size_t slot_bytes, foa_frame_result *d_results)
 {
+    AfterScope taken(rx);
     if (!rx) return fail(FOA_E_INVALID, "rx is NULL");
-    if (n_frames == 0) { rx->last_frames = 0; rx->after.clear(); return FOA_OK; }      // (nothing is queued: nothing waits)
+    if (n_frames == 0) { rx->last_frames = 0; return FOA_OK; }
     if (!d_iq || !d_descs || !d_ends || !d_psdu || !d_results) return fail(FOA_E_INVALID, "NULL device pointer");
     if (n_frames > 0x7FFFFFF0u || n_context > 0x7FFFFFF0u - n_frames) return fail(FOA_E_INVALID, "too many frames");
     HIP_TRY(enter_device(rx->device));
@@ -288,6 +290,7 @@ static int decode_frames_any(foa_rx *rx, const void *d_iq, bool f64, size_t n_sa
 static int decode_frames_host_any(foa_rx *rx, const void *iq, bool f64, size_t n_samples, const foa_frame_desc *descs, const int64_t *ends,
                                   size_t n_frames, uint8_t *psdu, size_t slot_bytes, foa_frame_result *results)
 {
+    AfterScope taken(rx);
     if (!rx) return fail(FOA_E_INVALID, "rx is NULL");
     if (n_frames == 0) return FOA_OK;
     if (!iq || !descs || !ends || !psdu || !results) return fail(FOA_E_INVALID, "NULL pointer");
@@ -340,6 +343,7 @@ int foa_rx_submit_host(foa_rx *rx, const float *iq, size_t n_samples, const foa_
 int foa_rx_submit_host_ctx(foa_rx *rx, const float *iq, size_t n_samples, const foa_frame_desc *descs, const int64_t *ends, size_t n_frames,
                            size_t n_context, size_t slot_bytes, uint64_t *ticket)
 {
+    AfterScope taken(rx);
     if (!rx || !ticket) return fail(FOA_E_INVALID, "NULL argument");
     if (n_frames == 0 || !iq || !descs || !ends) return fail(FOA_E_INVALID, "empty call or NULL pointer");
     HIP_TRY(enter_device(rx->device));

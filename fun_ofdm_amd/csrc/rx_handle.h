@@ -202,6 +202,18 @@ inline int wait_after(foa_rx *rx, hipStream_t st)
     return FOA_OK;
 }
 
+// ... and every entry point that waits for them takes them along whichever way it returns -- refused, failed half-way, nothing to do: the
+// library holds raw handles that the caller may destroy once the call is back, so none may be left for a later call to wait for.
+// (While a stream engine is open the list is empty -- foa_rx_after refuses, foa_stream_create took what was there -- and is only read here:
+// the engine's submitter thread looks at it too.)
+struct AfterScope {
+    foa_rx *const rx;
+    explicit AfterScope(foa_rx *r) : rx(r) {}
+    ~AfterScope() { if (rx && !rx->after.empty()) rx->after.clear(); }
+    AfterScope(const AfterScope &) = delete;
+    AfterScope &operator=(const AfterScope &) = delete;
+};
+
 // ---- rx_decode.hip ----
 int upload_tables_decode(const DeviceTables &t);
 int workspace(foa_rx *rx, size_t n_samples, size_t n_frames);           // sizes rx->w

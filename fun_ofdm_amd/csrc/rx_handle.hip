@@ -358,18 +358,16 @@ int foa_rx_record_done(foa_rx *rx, void *event)
 int foa_rx_decode_frames_dev_after(foa_rx *rx, void *inputs_ready, const float *d_iq, size_t n_samples, const foa_frame_desc *d_descs, const int64_t *d_ends,
                                    size_t n_frames, uint8_t *d_psdu, size_t slot_bytes, foa_frame_result *d_results)
 {
+    AfterScope taken(rx);                                              // (also when one event too many is what refuses the call)
     if (inputs_ready) { int rc = foa_rx_after(rx, inputs_ready); if (rc) return rc; }
-    const int rc = foa_rx_decode_frames_dev(rx, d_iq, n_samples, d_descs, d_ends, n_frames, d_psdu, slot_bytes, d_results);
-    if (rx) rx->after.clear();                                         // (a call refused before it queued anything leaves nothing behind)
-    return rc;
+    return foa_rx_decode_frames_dev(rx, d_iq, n_samples, d_descs, d_ends, n_frames, d_psdu, slot_bytes, d_results);
 }
 
 int foa_rx_sync_dev_begin_after(foa_rx *rx, void *inputs_ready, const float *d_iq, size_t n_samples, foa_frame_desc *d_descs, int64_t *d_ends, size_t cap)
 {
+    AfterScope taken(rx);
     if (inputs_ready) { int rc = foa_rx_after(rx, inputs_ready); if (rc) return rc; }
-    const int rc = foa_rx_sync_dev_begin(rx, d_iq, n_samples, d_descs, d_ends, cap);
-    if (rx) rx->after.clear();
-    return rc;
+    return foa_rx_sync_dev_begin(rx, d_iq, n_samples, d_descs, d_ends, cap);
 }
 
 int foa_rx_wait_age(foa_rx *rx, int age)

@@ -83,6 +83,7 @@ extern "C" {
 
 int foa_rx_sync_dev_begin(foa_rx *rx, const float *d_iq, size_t n_samples, foa_frame_desc *d_descs, int64_t *d_ends, size_t cap)
 {
+    AfterScope taken(rx);
     if (!rx || !d_iq || !d_descs || !d_ends) return fail(FOA_E_INVALID, "NULL argument");
     if (rx->open_stream) return fail(FOA_E_STATE, "a stream engine owns this handle (and its pre-sync scratch): destroy the stream first");
     if (rx->sy_open) return fail(FOA_E_STATE, "a pre-sync is already in flight on this handle: foa_rx_sync_dev_end first");
@@ -92,7 +93,7 @@ int foa_rx_sync_dev_begin(foa_rx *rx, const float *d_iq, size_t n_samples, foa_f
     if (!rx->sy_done) HIP_TRY(hipEventCreateWithFlags(&rx->sy_done, hipEventDisableTiming));
     rx->sy_pin[0] = rx->sy_pin[1] = rx->sy_pin[2] = rx->sy_pin[3] = 0;
     rx->sy_cap = cap; rx->sy_ccap = 0;
-    if (n_samples == 0 || cap == 0) { rx->sy_cap = 0; rx->sy_open = true; rx->after.clear(); return FOA_OK; }          // (nothing queued; _end reports 0)
+    if (n_samples == 0 || cap == 0) { rx->sy_cap = 0; rx->sy_open = true; return FOA_OK; }          // (nothing queued; _end reports 0)
     { int rc = sync_dev_issue(rx, d_iq, n_samples, d_descs, d_ends, cap, &rx->sy_ccap, rx->sync_origin, true); if (rc) return rc; }
     hipStream_t st = side_stream(rx);
     HIP_TRY(hipMemcpyAsync(rx->sy_pin, rx->sy_n.p, 4 * sizeof(int32_t), hipMemcpyDeviceToHost, st));
@@ -120,6 +121,7 @@ int foa_rx_sync_dev_end(foa_rx *rx, size_t *n_found)
 
 int foa_rx_sync_dev(foa_rx *rx, const float *d_iq, size_t n_samples, foa_frame_desc *d_descs, int64_t *d_ends, size_t cap, size_t *n_found)
 {
+    AfterScope taken(rx);
     if (!n_found) return fail(FOA_E_INVALID, "NULL argument");
     *n_found = 0;
     int rc = foa_rx_sync_dev_begin(rx, d_iq, n_samples, d_descs, d_ends, cap);

@@ -25,6 +25,7 @@ extern "C" {
 int foa_tx_build_frames_dev(foa_rx *rx, const uint8_t *d_payloads, size_t payload_pitch, int length, int rate, size_t n_frames,
                             double *d_frames, size_t *frame_samples)
 {
+    AfterScope taken(n_frames ? rx : nullptr);                         // (n_frames = 0 only asks for the size: the events stay for the call that builds)
     if (!rx || !frame_samples) return fail(FOA_E_INVALID, "NULL argument");
     if (rate < 0 || rate >= kNumRates || length < 0 || length > 4095) return fail(FOA_E_INVALID, "bad rate/length");
     DeviceTables tab;
@@ -53,6 +54,7 @@ int foa_tx_build_frames_dev(foa_rx *rx, const uint8_t *d_payloads, size_t payloa
 int foa_tx_channel_dev(foa_rx *rx, const double *d_frames, size_t n_frames, size_t frame_samples, size_t pitch, size_t lead, double snr_db,
                        double cfo_hz, uint64_t seed, float *d_iq)
 {
+    AfterScope taken(rx);
     if (!rx) return fail(FOA_E_INVALID, "rx is NULL");
     if (n_frames == 0) return FOA_OK;
     if (!d_frames || !d_iq) return fail(FOA_E_INVALID, "NULL device pointer");

@@ -307,6 +307,7 @@ extern "C" {
 
 int foa_stream_create(foa_rx *rx, size_t batch_samples, int narrow_threads, foa_stream **out)
 {
+    foa::AfterScope taken(rx);                       // (a stream reads host memory only: nothing of it waits for the caller's events)
     if (!rx || !out) return fail(FOA_E_INVALID, "NULL argument");
     *out = nullptr;
     if (batch_samples < 4096 || batch_samples > ((size_t)1 << 28)) return fail(FOA_E_INVALID, "batch_samples must lie in [4096, 2^28]");

@@ -234,7 +234,10 @@ int foa_rx_collect(foa_rx *rx, uint64_t ticket, int wait, uint8_t *psdu, foa_fra
  *                                   e -- recorded by the caller behind whatever produces that call's inputs and prepares its outputs (a
  *                                   fill of the PSDU slots, say).  One-shot; up to 16 events may be registered for one call.  The event must
  *                                   have been recorded, and must stay alive until that call has returned (the library keeps the handle, not
- *                                   a reference); a call that queues nothing (n_frames = 0) takes the registered events with it.
+ *                                   a reference).  That call takes the registered events with it whatever it returns: one that queues nothing
+ *                                   (n_frames = 0), is refused or fails leaves none for the next, so register them again before trying again.
+ *                                   foa_stream_create takes them too (a stream reads no device memory of the caller's); asking
+ *                                   foa_tx_build_frames_dev for a frame's size (n_frames = 0) does not.
  *   foa_rx_record_consumed(rx, e)   records e so that it completes when everything queued so far has READ what it reads of the caller's
  *                                   input buffers: the caller's stream waits for e (hipStreamWaitEvent) before it refills them.  Cheap.
  *   foa_rx_record_done(rx, e)       records e so that it completes when everything queued so far is complete (PSDU slots, results,
