@@ -29,6 +29,7 @@ class Receiver:
     def __init__(self, device=0):
         self._lib = lib()
         self._h = C.c_void_p()
+        self._after_keep = []                            # the events registered for the next call, alive until it is back (the library holds raw handles)
         self._check(self._lib.foa_rx_create(C.byref(self._h), int(device)))
         self.device = int(device)
         if self.notes():
@@ -37,6 +38,13 @@ class Receiver:
 
     def _check(self, rc):
         check(rc, self._lib)
+
+    def _take(self, fn, *args):
+        """A call of the library that takes the registered events with it, whatever it returns: only then are they let go."""
+        try:
+            self._check(fn(self._h, *args))
+        finally:
+            self._after_keep.clear()
 
     def close(self):
         if getattr(self, "_h", None):
@@ -57,13 +65,13 @@ class Receiver:
             return                                       # idle (the steady state of a loop that orders by other means): nothing to wait for
         ev = torch.cuda.Event()
         ev.record(s)
-        self._check(self._lib.foa_rx_after(self._h, ev.cuda_event))
-        self._after_keep = ev                            # (alive until the call below has queued its wait)
+        self.after(ev)
 
     def after(self, event):
-        """foa_rx_after: the next call that queues device work waits (on the device) for `event`, a torch.cuda.Event that has been recorded."""
+        """foa_rx_after: the next call that queues device work waits (on the device) for `event`, a torch.cuda.Event that has been recorded.
+        Up to 16 per call; the receiver keeps them alive until that call is back.  A call that is refused takes them with it too."""
         self._check(self._lib.foa_rx_after(self._h, event.cuda_event))
-        self._after_keep = event
+        self._after_keep.append(event)
 
     def record_consumed(self, event):
         """foa_rx_record_consumed: `event` (a torch.cuda.Event that has been recorded once, so that its handle exists) completes when everything
@@ -108,7 +116,7 @@ class Receiver:
         psdu = np.zeros((m, slot_bytes), np.uint8) if psdu_out is None else psdu_out
         assert psdu.shape == (m, slot_bytes) and psdu.dtype == np.uint8 and psdu.flags.c_contiguous
         res = np.zeros(m, frame_result_dtype)
-        self._check(self._lib.foa_rx_decode_frames_host(self._h, _vp(iq), iq.size, _vp(descs), _vp(ends), m, _vp(psdu), slot_bytes, _vp(res)))
+        self._take(self._lib.foa_rx_decode_frames_host, _vp(iq), iq.size, _vp(descs), _vp(ends), m, _vp(psdu), slot_bytes, _vp(res))
         return psdu, res
 
     def decode_frames_f64_host(self, iq_rotated, descs, ends, slot_bytes=4096):
@@ -119,7 +127,7 @@ class Receiver:
         m = descs.size
         psdu = np.zeros((m, slot_bytes), np.uint8)
         res = np.zeros(m, frame_result_dtype)
-        self._check(self._lib.foa_rx_decode_frames_f64_host(self._h, _vp(iq), iq.size, _vp(descs), _vp(ends), m, _vp(psdu), slot_bytes, _vp(res)))
+        self._take(self._lib.foa_rx_decode_frames_f64_host, _vp(iq), iq.size, _vp(descs), _vp(ends), m, _vp(psdu), slot_bytes, _vp(res))
         return psdu, res
 
     def submit_host(self, iq, descs, ends, slot_bytes=4096, n_context=0):
@@ -131,7 +139,7 @@ class Receiver:
         assert ends.size == descs.size and 0 <= n_context < max(descs.size, 1)
         t = C.c_uint64(0)
         m = descs.size - n_context
-        self._check(self._lib.foa_rx_submit_host_ctx(self._h, _vp(iq), iq.size, _vp(descs), _vp(ends), m, n_context, slot_bytes, C.byref(t)))
+        self._take(self._lib.foa_rx_submit_host_ctx, _vp(iq), iq.size, _vp(descs), _vp(ends), m, n_context, slot_bytes, C.byref(t))
         return (int(t.value), m, slot_bytes)
 
     def collect(self, ticket, wait=True):
@@ -161,8 +169,8 @@ class Receiver:
         m = ends.numel() - n_context - n_lead
         assert descs.numel() * descs.element_size() == ends.numel() * frame_desc_dtype.itemsize
         assert psdu.shape[0] == m and results.numel() == 4 * m
-        self._check(self._lib.foa_rx_decode_frames_lead_ctx_dev(self._h, iq.data_ptr(), n, descs.data_ptr(), ends.data_ptr(), n_lead, m, n_context, psdu.data_ptr(),
-                                                      psdu.shape[1], results.data_ptr()))
+        self._take(self._lib.foa_rx_decode_frames_lead_ctx_dev, iq.data_ptr(), n, descs.data_ptr(), ends.data_ptr(), n_lead, m, n_context, psdu.data_ptr(),
+                   psdu.shape[1], results.data_ptr())
 
     def sync_dev(self, iq, descs, ends):
         """Device-side frame_detector + timing_sync: iq complex64[n] (CUDA tensor), descs uint8[cap*48], ends int64[cap]
@@ -172,7 +180,7 @@ class Receiver:
         assert descs.numel() * descs.element_size() >= cap * frame_desc_dtype.itemsize
         self._after_torch(iq)
         got = C.c_size_t(0)
-        self._check(self._lib.foa_rx_sync_dev(self._h, iq.data_ptr(), n, descs.data_ptr(), ends.data_ptr(), cap, C.byref(got)))
+        self._take(self._lib.foa_rx_sync_dev, iq.data_ptr(), n, descs.data_ptr(), ends.data_ptr(), cap, C.byref(got))
         return int(got.value)
 
     def sync_dev_begin(self, iq, descs, ends):
@@ -181,7 +189,7 @@ class Receiver:
         cap = ends.numel()
         assert descs.numel() * descs.element_size() >= cap * frame_desc_dtype.itemsize
         self._after_torch(iq)
-        self._check(self._lib.foa_rx_sync_dev_begin(self._h, iq.data_ptr(), n, descs.data_ptr(), ends.data_ptr(), cap))
+        self._take(self._lib.foa_rx_sync_dev_begin, iq.data_ptr(), n, descs.data_ptr(), ends.data_ptr(), cap)
 
     def sync_dev_end(self):
         got = C.c_size_t(0)
@@ -202,7 +210,7 @@ class Receiver:
         out = torch.empty((n, s, 2), dtype=torch.float64, device=payloads.device)
         got = C.c_size_t(0)
         self._after_torch(payloads)
-        self._check(self._lib.foa_tx_build_frames_dev(self._h, payloads.data_ptr(), payloads.stride(0), int(length), int(rate), n, out.data_ptr(), C.byref(got)))
+        self._take(self._lib.foa_tx_build_frames_dev, payloads.data_ptr(), payloads.stride(0), int(length), int(rate), n, out.data_ptr(), C.byref(got))
         self.sync()
         return out
 
@@ -212,7 +220,7 @@ class Receiver:
         n, s, _ = frames.shape
         iq = torch.empty((n * pitch, 2), dtype=torch.float32, device=frames.device)
         self._after_torch(frames)
-        self._check(self._lib.foa_tx_channel_dev(self._h, frames.data_ptr(), n, s, int(pitch), int(lead), float(snr_db), float(cfo_hz), int(seed), iq.data_ptr()))
+        self._take(self._lib.foa_tx_channel_dev, frames.data_ptr(), n, s, int(pitch), int(lead), float(snr_db), float(cfo_hz), int(seed), iq.data_ptr())
         self.sync()
         return iq
 
@@ -296,7 +304,7 @@ class Stream:
         self._rx = receiver
         self._lib = receiver._lib
         self._h = C.c_void_p()
-        self._check(self._lib.foa_stream_create(receiver._h, int(batch_samples), int(narrow_threads), C.byref(self._h)))
+        receiver._take(self._lib.foa_stream_create, int(batch_samples), int(narrow_threads), C.byref(self._h))
 
     def _check(self, rc):
         check(rc, self._lib)
