@@ -114,7 +114,7 @@ struct foa_rx {
     hipStream_t stream3 = nullptr;     // pipelined path: copies of the host-pointer entry points and the pre-sync stage
     hipStream_t stream4 = nullptr;     // the second lane of pipelined calls (the first is `stream`)
     hipStream_t stream5 = nullptr, stream6 = nullptr;      // third and fourth lane, used for small grids (option "depth")
-    int max_depth = 4;                 // lanes that can run side by side (2 if the host cut the runtime down to one hardware queue per priority: foa_rx_create)
+    int max_depth = 4;                 // lanes that can run side by side (2 if the host cut the runtime down to fewer hardware queues: foa_rx_create)
     std::string notes;                 // non-fatal remarks about how the handle is set up (foa_rx_notes)
     int64_t sync_origin = 0;           // one-shot device pre-sync: stream index of d_iq[0] (option "sync_origin")
     int64_t stream_longest = 0;        // foa_stream_create: longest frame (samples, preamble to last symbol + 192) the stream will hold; 0 = any frame the format allows
@@ -167,7 +167,7 @@ struct foa_rx {
     size_t sy_cap = 0;
     // Device-side ordering against the caller's own streams (foa_rx_after / foa_rx_record_consumed / foa_rx_record_done):
     std::vector<hipEvent_t> after;     // events the NEXT call that queues work makes its first stream wait for (one-shot)
-    hipStream_t join = nullptr;        // made on first use, high priority: carries event waits and the caller's record, never a kernel
+    hipStream_t join = nullptr;        // made on first use: carries event waits and the caller's record, never a kernel
     hipEvent_t tx_done = nullptr;      // behind the most recent foa_tx_* call (they read caller buffers on `stream`)
     bool tx_used = false, sy_used = false;
     foa_stream *open_stream = nullptr;      // the stream engine that owns this handle right now (stream_engine.h), if any
@@ -179,7 +179,7 @@ namespace foa {
 // A machine that a call fills (config 2: five forward-pass waves per SIMD) is best served by two calls' loops in flight; a call of a few
 // thousand frames leaves most SIMDs one wave or none, its forward pass lasts as long as ONE wave needs for its frames' trellis steps
 // whatever the batch, and more loops in flight are what raises the throughput then (1 000 frames x 4 092 bytes at 54 Mbps: 1.43 ms per
-// batch with two, 0.94 with four).  The lanes sit on hardware queues of their own (stream priorities: foa_rx_create).
+// batch with two, 0.94 with four).  (foa_rx_create: how the lanes come by hardware queues.)
 constexpr int kDeepBelow = 4609;                 // frames: up to 2.25 forward-pass waves per SIMD.  (Round 5 drew the line at 2049; measured since: 3 000 frames per call
                                                  // +9 % with four loops, 4 000 mixed-rate alignments +14 %, 5 000 frames the same
                                                  // either way, 6 000 and more 2-8 % better with two: profiles/r06_depth_by_frames.txt)
@@ -189,8 +189,6 @@ constexpr int kSingleBelow = 2049;               // alignments: below this -- up
 inline bool piped(const foa_rx *rx) { return rx->pipeline; }
 // Host-pointer entry points copy their inputs (and the pre-sync stage runs) on the third stream when calls are pipelined, off the
 // lanes, so that a copy never sits behind a forward pass; the decode call that follows waits for the event.
-// the priority level of copy / pre-sync / look-ahead streams (foa_rx_create: hardware queues come in a pool per priority)
-inline int high_priority() { int least = 0, greatest = 0; (void)hipDeviceGetStreamPriorityRange(&least, &greatest); return greatest; }
 inline hipStream_t side_stream(foa_rx *rx) { return rx->pipeline ? rx->stream3 : rx->stream; }
 
 // foa_rx_after: whatever the caller registered is waited for by `st`, the stream the call's first kernel or copy goes to -- everything else

@@ -137,33 +137,30 @@ int foa_rx_create(foa_rx **out, int device)
     if (strncmp(prop.gcnArchName, "gfx950", 6) != 0) return fail(FOA_E_NO_DEVICE, "device %d is %s; this library is built for gfx950 only", device, prop.gcnArchName);
     foa_rx *rx = new foa_rx();
     rx->device = device;
-    // Six streams want six hardware queues that do not get in each other's way.  Two things decide that, both measured (tools/probe_queues.hip,
-    // tools/probe_pipes.hip, profiles/r05_ab_stream_layout_host_queues.txt):
-    //  * the runtime keeps a pool of GPU_MAX_HW_QUEUES hardware queues (default 4, read when it starts) PER STREAM PRIORITY and hands a new
-    //    stream the least used one once the pool is full.  Streams of the normal priority share the pool with whatever the host made;
+    // Six streams, every one at the DEFAULT priority: work on streams of different priorities side by side has hung these GPUs for good.  (The
+    // layout before this one made the lanes at the lowest level and the stitch and copy streams at the highest, for the hardware queues that
+    // come with it; figures measured under it are not this one's.)  What decides how they overlap, both measured (tools/probe_queues.hip,
+    // tools/probe_pipes.hip):
+    //  * the runtime keeps a pool of GPU_MAX_HW_QUEUES hardware queues (default 4, read when it starts) and hands a new stream the least used
+    //    one once the pool is full; the host's own streams are in the same pool.  Six streams on four queues share some of them: work that
+    //    shares a queue runs in the order it was queued, which is never wrong -- whatever an event waits for was queued before the wait;
     //  * a process's hardware queues go round the GPU's four dispatch pipes in the order they were made (queue k on pipe k mod 4), and a grid
     //    that does not fit on the machine at once -- the forward pass -- keeps its pipe busy until its last workgroup has started: another
-    //    queue on that pipe waits.  Two lanes, the stitch stream and the copy stream on two pipes run at 24-29 Gsample/s instead of 37,
-    //    which is what round 4's layout (six normal streams) did in a host that had made two or three streams of its own.
-    // So: no stream at the normal level.  The four lanes sit at the LOW level (the decode yields to the host's own normal-priority work), the
-    // stitch / CRC stream and the copy / pre-sync stream at the HIGH one (short kernels that gate the next call), and they are made in the
-    // order lane 1, stitch, copy, lane 2, lane 3, lane 4: four queues in a row are on four different pipes wherever the row starts.  Same
-    // speed with 0 .. 3 queues made by the host before, with the runtime's default of 4 queues and with 8; small batches no longer need
-    // GPU_MAX_HW_QUEUES=8 (1 000 frames per call: 9.2 -> 11.0 Gsample/s at the default).
+    //    queue on that pipe waits.
+    // So the four streams that a machine-filling call uses come first: lane 1, stitch / CRC, copy / pre-sync, lane 2 -- four queues in a row
+    // are on four different pipes wherever the row starts -- and the third and fourth lane of small calls behind them.
     {
-        int least = 0, greatest = 0;
-        HIP_TRY(hipDeviceGetStreamPriorityRange(&least, &greatest));         // (numerically greatest <= least)
-        HIP_TRY(hipStreamCreateWithPriority(&rx->stream, hipStreamNonBlocking, least));
-        HIP_TRY(hipStreamCreateWithPriority(&rx->stream2, hipStreamNonBlocking, greatest));
-        HIP_TRY(hipStreamCreateWithPriority(&rx->stream3, hipStreamNonBlocking, greatest));
-        HIP_TRY(hipStreamCreateWithPriority(&rx->stream4, hipStreamNonBlocking, least));
-        HIP_TRY(hipStreamCreateWithPriority(&rx->stream5, hipStreamNonBlocking, least));
-        HIP_TRY(hipStreamCreateWithPriority(&rx->stream6, hipStreamNonBlocking, least));
+        HIP_TRY(hipStreamCreateWithFlags(&rx->stream, hipStreamNonBlocking));
+        HIP_TRY(hipStreamCreateWithFlags(&rx->stream2, hipStreamNonBlocking));
+        HIP_TRY(hipStreamCreateWithFlags(&rx->stream3, hipStreamNonBlocking));
+        HIP_TRY(hipStreamCreateWithFlags(&rx->stream4, hipStreamNonBlocking));
+        HIP_TRY(hipStreamCreateWithFlags(&rx->stream5, hipStreamNonBlocking));
+        HIP_TRY(hipStreamCreateWithFlags(&rx->stream6, hipStreamNonBlocking));
         const char *q = getenv("GPU_MAX_HW_QUEUES");
-        if (q && atoi(q) < 4) {                                          // (also set but empty = 1) fewer queues per pool than lanes
+        if (q && atoi(q) < 4) {                                          // (also set but empty = 1) fewer queues than lanes
             rx->max_depth = 2;
             rx->notes += "GPU_MAX_HW_QUEUES is set below 4: the four lanes of small decode calls would share hardware queues, so such calls keep 2 loops in "
-                         "flight instead of 4; leave the variable unset (the runtime's default of 4 per priority level is enough). ";
+                         "flight instead of 4; leave the variable unset (the runtime's default is 4). ";
         }
     }
     HIP_TRY(hipEventCreateWithFlags(&rx->in_ready, hipEventDisableTiming));
@@ -291,7 +288,7 @@ int foa_rx_sync(foa_rx *rx)
 }
 
 // ---- device-side ordering against the caller's own streams --------------------------------------------------------------------------
-// The library's streams are its own (several, at other priorities than the host's): what orders them against a caller's stream is an
+// The library's streams are its own, several of them: what orders them against a caller's stream is an
 // event.  Nothing here makes the host wait.
 
 int foa_rx_after(foa_rx *rx, void *event)
@@ -304,10 +301,10 @@ int foa_rx_after(foa_rx *rx, void *event)
 }
 
 // the stream that joins the library's streams for a caller's event: made when first asked for (a handle that never orders against
-// a caller's stream keeps the queue layout of foa_rx_create), at the high priority level (it only ever carries waits and one record)
+// a caller's stream keeps the queue layout of foa_rx_create); it only ever carries waits and one record
 static int join_stream(foa_rx *rx)
 {
-    if (!rx->join) HIP_TRY(hipStreamCreateWithPriority(&rx->join, hipStreamNonBlocking, high_priority()));
+    if (!rx->join) HIP_TRY(hipStreamCreateWithFlags(&rx->join, hipStreamNonBlocking));
     return FOA_OK;
 }
 

@@ -339,7 +339,7 @@ int foa_stream_create(foa_rx *rx, size_t batch_samples, int narrow_threads, foa_
         if (!rc && hipEventCreateWithFlags(&g.in_done[i], hipEventDisableTiming) != hipSuccess) rc = fail(FOA_E_HIP, "hipEventCreate failed");
         if (!rc && hipEventCreateWithFlags(&g.sel_done[i], hipEventDisableTiming) != hipSuccess) rc = fail(FOA_E_HIP, "hipEventCreate failed");
     }
-    if (!rc && hipStreamCreateWithPriority(&g.st_in, hipStreamNonBlocking, high_priority()) != hipSuccess) rc = fail(FOA_E_HIP, "hipStreamCreate failed");
+    if (!rc && hipStreamCreateWithFlags(&g.st_in, hipStreamNonBlocking) != hipSuccess) rc = fail(FOA_E_HIP, "hipStreamCreate failed");
     if (!rc && hipHostMalloc((void **)&g.sel, (size_t)foa::kStreamBufs * 8 * sizeof(int32_t), hipHostMallocDefault) != hipSuccess) rc = fail(FOA_E_NOMEM, "hipHostMalloc failed");
     if (!rc) rc = g.sel_dev.ensure((size_t)foa::kStreamBufs * 8);
     if (!rc) rc = g.la_range.ensure((size_t)foa::kStreamBufs * 2);

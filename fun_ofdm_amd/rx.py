@@ -54,7 +54,7 @@ class Receiver:
     __del__ = close
 
     def _after_torch(self, t):
-        """The library's streams know nothing of torch's (and run at other priorities): before a call that reads or writes torch tensors,
+        """The library's streams know nothing of torch's: before a call that reads or writes torch tensors,
         whatever torch's CURRENT stream on the tensor's device still has queued -- the copy that made an input, the fill of an output
         tensor -- must be through.  Ordered on the DEVICE (foa_rx_after with an event recorded on that stream): the host does not wait.
         Work the caller has queued on OTHER torch streams (a side stream, a non_blocking copy stream) is not covered: record an event
@@ -159,7 +159,7 @@ class Receiver:
         psdu uint8[m, slot]; results int32[m, 4].  n_lead: the first alignments of descs / ends were decided by an earlier piece
         (looked at only for where they sit); n_context: the last ones are context only (foa_rx_decode_frames_lead_ctx_dev).
         Asynchronous on the handle's streams, which are NOT ordered against
-        torch's (and run at other priorities: a fill torch has queued for an output tensor may land after the kernels
+        torch's (a fill torch has queued for an output tensor may land after the kernels
         that write it), so the wrapper makes the call wait, on the device, for what torch's current stream has queued
         (_after_torch -> foa_rx_after).  settle=False: the
         caller orders torch's work on these tensors against the call itself (bench.py's loop does, with one event per output set)."""

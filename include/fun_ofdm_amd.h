@@ -83,18 +83,16 @@ const char *foa_last_error(void);
 int foa_device_count(void);
 
 /* The library runs a call's stages on up to six HIP streams (two to four lanes of pipelined decode calls, one for the stitch / CRC
- * kernels, one for copies and the pre-sync).  Streams overlap when they sit on different hardware queues, and big grids only when those
- * queues sit on different dispatch pipes.  The HIP runtime keeps a pool of GPU_MAX_HW_QUEUES queues (default 4, fixed when it starts) per
- * stream PRIORITY, and a process's queues go round the four pipes in the order they were made; so the library makes its lanes at the LOW
- * priority level and its stitch and copy streams at the HIGH one, in an order that puts any four in a row on four pipes -- none at the
- * normal level, where the host's own streams live.  It runs at full speed with the runtime's defaults and whatever streams the host has
- * made (profiles/r05_ab_stream_layout_host_queues.txt); the host sets nothing (rounds 3-4 asked for GPU_MAX_HW_QUEUES=8, and lost a
- * third of their speed behind two host streams).  The decode therefore yields to normal-priority work of the host on the same GPU.
- * Only a host that sets GPU_MAX_HW_QUEUES below 4 is told so by foa_rx_notes(). */
+ * kernels, one for copies and the pre-sync), all non-blocking and all at the DEFAULT priority: streams of different priorities side by
+ * side have hung these GPUs, so a host should keep its own at the default too.  Streams overlap when they sit on different hardware queues,
+ * and big grids only when those queues sit on different dispatch pipes.  The HIP runtime keeps a pool of GPU_MAX_HW_QUEUES queues
+ * (default 4, fixed when it starts) that the library shares with the host's streams, and a process's queues go round the four pipes in the
+ * order they were made; the library makes the four streams of a machine-filling call first, one after the other.  Which streams share a
+ * queue never changes a result, only how much overlaps.  A host that sets GPU_MAX_HW_QUEUES below 4 is told so by foa_rx_notes(). */
 
 /* Create a receiver on HIP device `device` (its own non-blocking streams). */
 int foa_rx_create(foa_rx **out, int device);
-/* Non-fatal remarks about how the handle is set up ("" if none), e.g. a runtime cut down to fewer hardware queues per priority than the library has lanes.  Valid until the handle
+/* Non-fatal remarks about how the handle is set up ("" if none), e.g. a runtime cut down to fewer hardware queues than the library has lanes.  Valid until the handle
  * is destroyed. */
 const char *foa_rx_notes(foa_rx *rx);
 void foa_rx_destroy(foa_rx *rx);
@@ -115,7 +113,7 @@ int foa_rx_reserve(foa_rx *rx, size_t n_samples, size_t n_frames);
  *                 stream.  (Waits for everything in flight before it switches.)
  *   "depth"       pipelined calls: how many calls' loops are in flight -- 0 (default) = by grid size: 2 (3 for BPSK-only captures: option "max_dbps" <= 36), or 4 for calls of up to 4608 frames,
  *                 whose forward pass leaves most SIMDs a single wave (1 000-frame batches decode 40-50 % faster in steady state); 2, 3, 4 =
- *                 fixed.  (the lanes sit on hardware queues of their own: stream priorities, see above)
+ *                 fixed.  (the lanes share the process's hardware queues, see above)
  *   "max_dbps"    what the work sets of later calls (and foa_rx_reserve) are sized for: the data bits per OFDM symbol of the HIGHEST rate the
  *                 caller's frames carry, 24 (6 Mbps) .. 216 (54 Mbps, the default: any rate).  A call's per-step buffers -- 10.25 bytes per
  *                 trellis step, several sets in rotation -- hold n_samples / 80 x max_dbps steps, so a capture of 6 Mbps frames needs a
@@ -246,9 +244,8 @@ int foa_rx_collect(foa_rx *rx, uint64_t ticket, int wait, uint8_t *psdu, foa_fra
  *   foa_rx_decode_frames_dev_after / foa_rx_sync_dev_begin_after = foa_rx_after(rx, inputs_ready) + the call (inputs_ready may be NULL).
  *
  * A capture loop over two device buffers with no host synchronisation in it: INTEGRATION.md 2; tests/cpp/test_ordering.cpp runs one
- * against the oracle.  The library's lanes run BELOW the normal stream priority and its short stitch / copy streams above (see the
- * top of this file), so an un-ordered producer on a normal-priority stream is overtaken in both directions: order with these calls, or
- * complete the buffers before the call. */
+ * against the oracle.  The library's streams are non-blocking and know nothing of the caller's, so an un-ordered producer is overtaken
+ * in both directions: order with these calls, or complete the buffers before the call. */
 int foa_rx_after(foa_rx *rx, void *event);
 int foa_rx_record_consumed(foa_rx *rx, void *event);
 int foa_rx_record_done(foa_rx *rx, void *event);

@@ -26,3 +26,7 @@ def build_and_run(tmp_path, name):
 
 def test_a_call_takes_the_registered_events_with_it_whatever_it_returns(tmp_path):
     assert "all checks passed" in build_and_run(tmp_path, "after_events")
+
+
+def test_every_stream_has_the_default_priority(tmp_path):
+    assert "all checks passed" in build_and_run(tmp_path, "stream_priorities")

@@ -2,15 +2,14 @@
 // side (probe_queues.hip), but a grid that does not fit on the machine at once keeps its queue's dispatcher busy until its last workgroup
 // has started, and a kernel on another queue served by the same dispatcher waits for that.  Two pipelined decode lanes placed like that run
 // one after the other (profiles/r05_ab_stream_layout.txt: 27.7 against 37.2 Gsample/s, decided by the ORDER in which six streams were created).
-// Here: S streams are created in order (priorities given on the command line, default all normal); for every ordered pair (i, j) a BIG grid
+// Here: S streams are created in order, all at the default priority; for every ordered pair (i, j) a BIG grid
 // (4 096 workgroups, two resident per CU through their LDS, ~4 ms) goes to stream i and one single-wave kernel (~0.2 ms) to stream j; the
 // time until the small one is done says whether j had to wait for i's dispatch.
-//   hipcc --offload-arch=gfx950 -O3 -o build/probe_pipes.bin tools/probe_pipes.hip ;  build/probe_pipes.bin [S] [priority pattern, e.g. 0,-1,-1,0,1,1]
+//   hipcc --offload-arch=gfx950 -O3 -o build/probe_pipes.bin tools/probe_pipes.hip ;  build/probe_pipes.bin [S]
 #include <hip/hip_runtime.h>
 #include <chrono>
 #include <cstdio>
 #include <cstdlib>
-#include <cstring>
 #include <vector>
 
 __global__ void k_big(unsigned long long ticks, unsigned long long *out)
@@ -32,15 +31,11 @@ __global__ void k_small(unsigned long long ticks, unsigned long long *out)
 int main(int argc, char **argv)
 {
     const int S = argc > 1 ? atoi(argv[1]) : 12;
-    std::vector<int> prio(S, 0);
-    if (argc > 2) { char *p = strtok(argv[2], ","); for (int i = 0; i < S && p; i++, p = strtok(nullptr, ",")) prio[i] = atoi(p); }
     const char *q = getenv("GPU_MAX_HW_QUEUES");
-    printf("GPU_MAX_HW_QUEUES %s; %d streams, priorities:", q ? q : "(unset: 4)", S);
-    for (int i = 0; i < S; i++) printf(" %d", prio[i]);
-    printf("\n");
+    printf("GPU_MAX_HW_QUEUES %s; %d streams\n", q ? q : "(unset: 4)", S);
     (void)hipFuncSetAttribute((const void *)k_big, hipFuncAttributeMaxDynamicSharedMemorySize, 65536);
     std::vector<hipStream_t> st(S);
-    for (int i = 0; i < S; i++) (void)hipStreamCreateWithPriority(&st[i], hipStreamNonBlocking, prio[i]);
+    for (int i = 0; i < S; i++) (void)hipStreamCreateWithFlags(&st[i], hipStreamNonBlocking);
     unsigned long long *d;
     (void)hipMalloc(&d, 64 * sizeof *d);
     const unsigned long long big_ticks = 1200000, small_ticks = 480000;  // the counter runs at ~2.4 GHz: 0.5 ms per workgroup (x 8 rounds), 0.2 ms
