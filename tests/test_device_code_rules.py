@@ -4,7 +4,9 @@ Writes through the scalar data cache (scalar stores, scalar atomics, that cache'
 shared GPUs, comments included: data is written with vector stores.  The patterns below are put together from pieces so that this file does
 not hold the words itself.
 
-Streams are made at the default priority: streams of different priorities side by side have hung these GPUs for good."""
+Streams are made at the default priority: streams of different priorities side by side have hung these GPUs for good.
+
+No packed fp32 arithmetic: some forms of it have given wrong results on this hardware, and the compiler makes it by itself unless told not to."""
 import os
 import re
 import shutil
@@ -81,4 +83,20 @@ def test_no_source_makes_a_stream_of_another_priority():
         for n, line in enumerate(open(path, errors="replace"), 1):
             if PRIORITY_STREAM.search(line):
                 bad.append("%s:%d" % (os.path.relpath(path, ROOT), n))
+    assert not bad, bad
+
+
+NO_PACKED = "-Xclang -target-feature -Xclang -packed-fp32-ops"
+
+
+def test_every_unit_is_compiled_without_packed_fp32():
+    out = subprocess.run(["make", "-n", "-B", "-C", os.path.join(ROOT, "fun_ofdm_amd", "csrc")], check=True, capture_output=True, text=True).stdout
+    lines = [x for x in out.splitlines() if "hipcc" in x and " -c " in x]
+    assert len(lines) == 6 and all(NO_PACKED in x for x in lines), lines
+    variant = [x for x in open(os.path.join(ROOT, "tools", "variant.sh")) if "hipcc" in x and " -c " in x]
+    assert len(variant) == 1 and NO_PACKED in variant[0]
+
+
+def test_no_kernel_holds_packed_fp32_arithmetic(tmp_path):
+    bad = {m: n for m, n in device_code(tmp_path).items() if re.match(r"v_pk_(?:add|mul|fma)_f32", m)}
     assert not bad, bad

@@ -8,7 +8,7 @@ rm -rf $obj build/var_$name.so          # never link a stale object of an earlie
 mkdir -p $obj
 pids=()
 for u in rx_handle rx_decode rx_sync rx_stage rx_tx rx_stream; do
-  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-function "$@" -c -o $obj/$u.o $src/$u.hip &
+  /opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -std=c++17 -fPIC -Wno-unused-function -Xclang -target-feature -Xclang -packed-fp32-ops "$@" -c -o $obj/$u.o $src/$u.hip &
   pids+=($!)
 done
 for p in "${pids[@]}"; do wait $p || { echo "variant $name: a unit failed to compile" >&2; exit 1; }; done
