@@ -303,6 +303,8 @@ static int decode_frames_host_any(foa_rx *rx, const void *iq, bool f64, size_t n
     if (rc) return rc;
     uint8_t *b = rx->scratch.p;
     hipStream_t st = side_stream(rx);
+    // (frames that a transmit call is still building read the same buffer on the handle's first stream: rx_tx.hip)
+    if (rx->tx_used && st != rx->stream) HIP_TRY(hipStreamWaitEvent(st, rx->tx_done, 0));
     if ((rc = wait_after(rx, st))) return rc;
     HIP_TRY(hipMemcpyAsync(b + o_iq, iq, n_samples * sample_bytes, hipMemcpyHostToDevice, st));
     HIP_TRY(hipMemcpyAsync(b + o_desc, descs, n_frames * sizeof(foa_frame_desc), hipMemcpyHostToDevice, st));

@@ -30,3 +30,7 @@ def test_a_call_takes_the_registered_events_with_it_whatever_it_returns(tmp_path
 
 def test_every_stream_has_the_default_priority(tmp_path):
     assert "all checks passed" in build_and_run(tmp_path, "stream_priorities")
+
+
+def test_a_host_decode_copies_its_inputs_behind_the_frames_being_built(tmp_path):
+    assert "all checks passed" in build_and_run(tmp_path, "scratch_order")
