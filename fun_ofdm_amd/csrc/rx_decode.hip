@@ -50,7 +50,7 @@ int foa::inputs_queued(foa_rx *rx, hipStream_t cs)
 {
     if (cs == rx->stream) return FOA_OK;
     HIP_TRY(hipEventRecord(rx->in_ready, cs));
-    rx->in_wait = true;
+    rx->in_wait = rx->side_work = true;
     return FOA_OK;
 }
 
@@ -99,7 +99,7 @@ int foa::flush_pending(foa_rx *rx, hipEvent_t after_front_end)
     HIP_TRY(hipEventRecord(p.w->done, sb));
     // (the one-shot pre-sync goes behind this walk -- rx_sync.hip -- when two loops are in flight: the walk is then about to run.  With
     // three or four loops it waits for a forward pass that has two or three others in front of it, and a pre-sync behind it would hold up
-    // the host, which needs the count to queue the next call: BASELINE config 5, 55 -> 52 Gsample/s)
+    // the host, which needs the count to queue the next call)
     rx->last_walk_done = p.deep ? nullptr : p.w->walk_done;
     if (p.job) {
         HostJob &j = *p.job;
@@ -202,15 +202,17 @@ static int decode_frames_any(foa_rx *rx, const void *d_iq, bool f64, size_t n_sa
     }
     int rc = workspace(rx, n_samples, n_frames + n_context);
     if (rc) return rc;
-    // Pipelined calls take turns on two (or four) streams ("lanes"): a call's front end, forward pass and chain-back walk run on ONE
+    // Pipelined calls take turns on two (to four) streams ("lanes"): a call's front end, forward pass and chain-back walk run on ONE
     // stream, the front end behind the walk of the call `depth` back (queued there when the call before this one was made).  The loop
     // that sets the step -- forward pass k, walk k, header, scan and data symbols of call k+2, forward pass k+2 -- is then one in-order
     // stream with no event packet in it, and nothing orders one lane behind the other (each call has its own work set), so a forward
     // pass starts the moment its front end is done, into the tail of the one before.
     // (big grids of BPSK-only captures -- the caller has said so: option "max_dbps" <= 36 -- spend a third of their time in the data-symbol
     // kernel, which shares the vector pipes with the forward pass: three loops keep a forward pass on the machine while two front ends
-    // run, + 8-11 % at 6 / 9 Mbps; from QPSK on it is within 3 % either way and config 2 loses 12 % to a third loop: profiles/r06_depth_by_frames.txt)
-    const int depth = rx->depth > 0 ? rx->depth : (n_frames < (size_t)kDeepBelow ? std::min(4, rx->max_depth) : (rx->max_dbps <= 36 ? std::min(3, rx->max_depth) : 2));
+    // run -- 5 120 frames of 4 092 bytes at 6 Mbps 4.52 -> 4.33 ms -- where config 2 loses 6 % to a third loop: profiles/stream_order.txt)
+    const bool third = !rx->side_work && !rx->sy_open && (n_frames < (size_t)kDeepBelow || rx->max_dbps <= 36);
+    const int depth = rx->depth > 0 ? rx->depth : third ? std::min(3, rx->max_depth) : 2;
+    rx->side_work = false;
     hipStream_t st = piped ? lane_stream(rx, (int)(rx->n_calls++ % (unsigned)depth)) : rx->stream;
     if (!piped && rx->prev->used && rx->prev != rx->w) HIP_TRY(hipStreamWaitEvent(st, rx->prev->done, 0));
     const int nf = (int)n_frames, n_total = (int)(n_frames + n_context);      // context alignments: header kernel only

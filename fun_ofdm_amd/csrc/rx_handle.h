@@ -113,12 +113,12 @@ struct foa_rx {
     hipStream_t stream2 = nullptr;     // pipelined path: the stitch / CRC kernel behind a call's chain-back walk
     hipStream_t stream3 = nullptr;     // pipelined path: copies of the host-pointer entry points and the pre-sync stage
     hipStream_t stream4 = nullptr;     // the second lane of pipelined calls (the first is `stream`)
-    hipStream_t stream5 = nullptr, stream6 = nullptr;      // third and fourth lane, used for small grids (option "depth")
+    hipStream_t stream5 = nullptr, stream6 = nullptr;      // third and fourth lane, used for small grids and a stream engine's small batches (option "depth")
     int max_depth = 4;                 // lanes that can run side by side (2 if the host cut the runtime down to fewer hardware queues: foa_rx_create)
     std::string notes;                 // non-fatal remarks about how the handle is set up (foa_rx_notes)
     int64_t sync_origin = 0;           // one-shot device pre-sync: stream index of d_iq[0] (option "sync_origin")
     int64_t stream_longest = 0;        // foa_stream_create: longest frame (samples, preamble to last symbol + 192) the stream will hold; 0 = any frame the format allows
-    int depth = 0;                     // how many calls' loops are in flight; 0 = by grid size (2, or 4 below kDeepBelow frames)
+    int depth = 0;                     // how many calls' loops are in flight; 0 = by grid size (2, or 3 below kDeepBelow frames)
     int depth_saved = -1;              // (the stream engine pins its own while a stream is open and restores this)
     unsigned n_calls = 0;              // pipelined decode calls made so far (a call's lane is n_calls mod depth)
     int q4_resident = 0;               // workgroups of the data-symbol kernel the device holds at once (its grid: rx_decode.hip)
@@ -132,6 +132,7 @@ struct foa_rx {
     bool record_soft = true;     // (the soft bytes are the front end's output and always there; the option is accepted for compatibility)
     hipEvent_t in_ready = nullptr;     // inputs copied by a host-pointer entry point are on the device (recorded on the copy stream)
     bool in_wait = false;              // ... and the next decode call's front end has to wait for that
+    bool side_work = false;            // copies or a pre-sync were queued on stream3 since the last decode call (they share lane 3's hardware queue: kDeepBelow)
     int64_t sync_call = 4096;    // pre-sync: the reference receiver's call size to decide timing_sync.cpp:99 by (sync_host.h kSyncCallDefault); 0 = as one call
     foa::WorkSet sets[foa::kSets];   // up to depth + 1 are in use at any time; one more keeps the call before them readable (timings)
     foa::WorkSet *w = &sets[0];      // the set of the most recent decode call
@@ -178,11 +179,12 @@ namespace foa {
 
 // A machine that a call fills (config 2: five forward-pass waves per SIMD) is best served by two calls' loops in flight; a call of a few
 // thousand frames leaves most SIMDs one wave or none, its forward pass lasts as long as ONE wave needs for its frames' trellis steps
-// whatever the batch, and more loops in flight are what raises the throughput then (1 000 frames x 4 092 bytes at 54 Mbps: 1.43 ms per
-// batch with two, 0.94 with four).  (foa_rx_create: how the lanes come by hardware queues.)
-constexpr int kDeepBelow = 4609;                 // frames: up to 2.25 forward-pass waves per SIMD.  (Round 5 drew the line at 2049; measured since: 3 000 frames per call
-                                                 // +9 % with four loops, 4 000 mixed-rate alignments +14 %, 5 000 frames the same
-                                                 // either way, 6 000 and more 2-8 % better with two: profiles/r06_depth_by_frames.txt)
+// whatever the batch, and more loops in flight are what raises the throughput then.  Three, not four: the fourth lane's hardware queue is
+// the stitch stream's (foa_rx_create).  Not where copies or a pre-sync were queued on stream3 since the last call: they share the third
+// lane's queue, so that call keeps two.
+constexpr int kDeepBelow = 6145;                 // frames: up to three forward-pass waves per SIMD.  ms per call at 54 Mbps with two | three loops in flight: 1 000 frames 0.30 | 0.24,
+                                                 // 3 000 0.49 | 0.38, 5 000 0.63 | 0.57, 6 000 0.67 | 0.64, 8 000 0.83 | 0.83, 10 000 0.97 | 1.02 (24 Mbps: 4 000 0.57 | 0.52,
+                                                 // 6 000 0.73 | 0.73, 8 000 0.90 | 0.95); pre-sync + decode of 4 000 at 24 Mbps 0.61 | 0.71: profiles/stream_order.txt
 constexpr int kSmallCallSegment = 192;           // chain-back segment of a call of up to 256 alignments: a lane walks segment + run-in steps one after the other, and such a call waits for exactly that
 constexpr int kSingleBelow = 2049;               // alignments: below this -- up to two four-wave workgroups per CU -- the forward pass takes one frame per wave (launch_fwd3)
 

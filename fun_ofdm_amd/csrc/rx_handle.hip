@@ -139,24 +139,38 @@ int foa_rx_create(foa_rx **out, int device)
     rx->device = device;
     // Six streams, every one at the DEFAULT priority: work on streams of different priorities side by side has hung these GPUs for good.  (The
     // layout before this one made the lanes at the lowest level and the stitch and copy streams at the highest, for the hardware queues that
-    // come with it; figures measured under it are not this one's.)  What decides how they overlap, both measured (tools/probe_queues.hip,
-    // tools/probe_pipes.hip):
-    //  * the runtime keeps a pool of GPU_MAX_HW_QUEUES hardware queues (default 4, read when it starts) and hands a new stream the least used
-    //    one once the pool is full; the host's own streams are in the same pool.  Six streams on four queues share some of them: work that
-    //    shares a queue runs in the order it was queued, which is never wrong -- whatever an event waits for was queued before the wait;
+    // come with it; figures measured under it are not this one's.)  What decides how they overlap, all measured (tools/probe_queues.hip,
+    // tools/probe_pipes.hip, profiles/stream_order.txt):
+    //  * the runtime keeps a pool of GPU_MAX_HW_QUEUES hardware queues (default 4, read when it starts): while the pool is not full a new
+    //    stream gets a queue of its own, after that the least used one, so that streams go round the queues in one fixed order.  The host's own
+    //    streams are in the same pool.  Work that shares a queue runs in the order it was queued, which is never wrong -- whatever an event
+    //    waits for was queued before the wait -- but a lane that shares with another lane is no second lane;
     //  * a process's hardware queues go round the GPU's four dispatch pipes in the order they were made (queue k on pipe k mod 4), and a grid
     //    that does not fit on the machine at once -- the forward pass -- keeps its pipe busy until its last workgroup has started: another
     //    queue on that pipe waits.
-    // So the four streams that a machine-filling call uses come first: lane 1, stitch / CRC, copy / pre-sync, lane 2 -- four queues in a row
-    // are on four different pipes wherever the row starts -- and the third and fourth lane of small calls behind them.
+    // So the pool is filled first, with streams that go again below: from then on any four streams made in a row sit on four queues, whatever the
+    // host made before (without that, 10 000 frames per call at 54 Mbps took 0.98 ms, or 1.22, or 1.43, by the number of host streams).
+    // Of the six, made in the order below, the first and the fifth share a queue and the second and the sixth: lane 4 with stitch / CRC, lane 3
+    // with copy / pre-sync.  Lanes 1 and 2, stitch and copy have a queue each (a machine-filling call: 0.98 ms), lanes 1, 2, 3 and stitch have
+    // (1 000 frames per call: 0.24 ms with three loops; 0.30 with lane 3 behind lane 1), and so have the four lanes (a stream of 4 Ki-sample
+    // batches keeps up with the air, 18.7 of 20 Msample/s with a lane behind another).
     {
-        HIP_TRY(hipStreamCreateWithFlags(&rx->stream, hipStreamNonBlocking));
-        HIP_TRY(hipStreamCreateWithFlags(&rx->stream2, hipStreamNonBlocking));
-        HIP_TRY(hipStreamCreateWithFlags(&rx->stream3, hipStreamNonBlocking));
-        HIP_TRY(hipStreamCreateWithFlags(&rx->stream4, hipStreamNonBlocking));
-        HIP_TRY(hipStreamCreateWithFlags(&rx->stream5, hipStreamNonBlocking));
-        HIP_TRY(hipStreamCreateWithFlags(&rx->stream6, hipStreamNonBlocking));
         const char *q = getenv("GPU_MAX_HW_QUEUES");
+        struct Fill {
+            std::vector<hipStream_t> s;
+            ~Fill() { for (auto st : s) (void)hipStreamDestroy(st); }
+        } fill;
+        for (int i = q ? std::min(std::max(atoi(q), 1), 32) : 4; i > 0; i--) {
+            hipStream_t st = nullptr;
+            HIP_TRY(hipStreamCreateWithFlags(&st, hipStreamNonBlocking));
+            fill.s.push_back(st);
+        }
+        HIP_TRY(hipStreamCreateWithFlags(&rx->stream6, hipStreamNonBlocking));      // lane 4
+        HIP_TRY(hipStreamCreateWithFlags(&rx->stream5, hipStreamNonBlocking));      // lane 3
+        HIP_TRY(hipStreamCreateWithFlags(&rx->stream, hipStreamNonBlocking));       // lane 1
+        HIP_TRY(hipStreamCreateWithFlags(&rx->stream4, hipStreamNonBlocking));      // lane 2
+        HIP_TRY(hipStreamCreateWithFlags(&rx->stream2, hipStreamNonBlocking));      // stitch / CRC
+        HIP_TRY(hipStreamCreateWithFlags(&rx->stream3, hipStreamNonBlocking));      // copies / pre-sync
         if (q && atoi(q) < 4) {                                          // (also set but empty = 1) fewer queues than lanes
             rx->max_depth = 2;
             rx->notes += "GPU_MAX_HW_QUEUES is set below 4: the four lanes of small decode calls would share hardware queues, so such calls keep 2 loops in "

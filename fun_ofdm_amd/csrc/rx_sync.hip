@@ -95,6 +95,7 @@ int foa_rx_sync_dev_begin(foa_rx *rx, const float *d_iq, size_t n_samples, foa_f
     rx->sy_cap = cap; rx->sy_ccap = 0;
     if (n_samples == 0 || cap == 0) { rx->sy_cap = 0; rx->sy_open = true; return FOA_OK; }          // (nothing queued; _end reports 0)
     { int rc = sync_dev_issue(rx, d_iq, n_samples, d_descs, d_ends, cap, &rx->sy_ccap, rx->sync_origin, true); if (rc) return rc; }
+    rx->side_work = true;
     hipStream_t st = side_stream(rx);
     HIP_TRY(hipMemcpyAsync(rx->sy_pin, rx->sy_n.p, 4 * sizeof(int32_t), hipMemcpyDeviceToHost, st));
     HIP_TRY(hipEventRecord(rx->sy_done, st));

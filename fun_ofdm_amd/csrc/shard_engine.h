@@ -59,8 +59,7 @@ struct ShardDev {
             if (!rc && hipEventCreateWithFlags(&sel_done[i], hipEventDisableTiming) != hipSuccess) rc = fail(FOA_E_HIP, "hipEventCreate failed");
             if (!rc && hipEventCreateWithFlags(&sync_done[i], hipEventDisableTiming) != hipSuccess) rc = fail(FOA_E_HIP, "hipEventCreate failed");
         }
-        // (the look-ahead stream first: made right behind the handle's six it lands on the pipe of the handle's copy / pre-sync stream, the
-        // staging stream on that of lane 2, whose forward pass holds its pipe for a millisecond at a time -- rx_handle.hip, foa_rx_create)
+        // (made behind the handle's six, these two share hardware queues with streams of it: rx_handle.hip, foa_rx_create)
         if (!rc && hipStreamCreateWithFlags(&st_sel, hipStreamNonBlocking) != hipSuccess) rc = fail(FOA_E_HIP, "hipStreamCreate failed");
         if (!rc && hipStreamCreateWithFlags(&st_in, hipStreamNonBlocking) != hipSuccess) rc = fail(FOA_E_HIP, "hipStreamCreate failed");
         if (!rc && hipHostMalloc((void **)&sel, (size_t)foa::kStreamBufs * 8 * sizeof(int32_t), hipHostMallocDefault) != hipSuccess) rc = fail(FOA_E_NOMEM, "hipHostMalloc failed");

@@ -375,8 +375,9 @@ int foa_stream_create(foa_rx *rx, size_t batch_samples, int narrow_threads, foa_
     // How many decode calls' loops in flight?  A batch of a million samples and more fills the machine with its forward pass: two (2.2
     // against 2.0 Gsample/s through process_samples with four).  A SMALL batch is a handful of forward-pass waves, and one wave walks its
     // frames' trellis at the lone-wave rate (0.65 ms for a 1024-byte frame at 54 Mbps) whatever the batch: what sets the rate of 64 Ki-sample
-    // batches is loops in flight over that latency -- 0.36 ms per batch with two -- so batches below a million samples get four where the
-    // runtime has the hardware queues for them (foa_rx_create).  FOA_STREAM_DEPTH overrides (A/B).
+    // batches is loops in flight over that latency, so batches below a million samples get four where the runtime has the hardware queues
+    // for them (foa_rx_create): 4 Ki-sample batches keep up with the air's 20 Msample/s with four and reach 18.8 with three, 64 Ki-sample
+    // ones run at 313 Msample/s against 260 (profiles/stream_order.txt).  FOA_STREAM_DEPTH overrides (A/B).
     rx->finish_in_line = batch_samples >= 8192 && batch_samples <= ((size_t)1 << 16) && !getenv("FOA_STREAM_FINISH_STITCH");
     rx->timing = false;                              // (nobody reads per-kernel times of a stream's batches: seven runtime calls less per batch)
     rx->depth_saved = rx->depth;

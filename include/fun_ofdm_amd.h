@@ -87,8 +87,10 @@ int foa_device_count(void);
  * side have hung these GPUs, so a host should keep its own at the default too.  Streams overlap when they sit on different hardware queues,
  * and big grids only when those queues sit on different dispatch pipes.  The HIP runtime keeps a pool of GPU_MAX_HW_QUEUES queues
  * (default 4, fixed when it starts) that the library shares with the host's streams, and a process's queues go round the four pipes in the
- * order they were made; the library makes the four streams of a machine-filling call first, one after the other.  Which streams share a
- * queue never changes a result, only how much overlaps.  A host that sets GPU_MAX_HW_QUEUES below 4 is told so by foa_rx_notes(). */
+ * order they were made.  foa_rx_create fills the pool (streams that it destroys again) before it makes its own, in an order that gives the
+ * streams that must overlap a queue each, whatever streams the host made before: lanes 1 and 2, stitch and copies for machine-filling
+ * calls, lanes 1 to 3 and stitch for small ones.  Which streams share a queue never changes a result, only how much overlaps.  A host that
+ * sets GPU_MAX_HW_QUEUES below 4 is told so by foa_rx_notes(). */
 
 /* Create a receiver on HIP device `device` (its own non-blocking streams). */
 int foa_rx_create(foa_rx **out, int device);
@@ -111,9 +113,9 @@ int foa_rx_reserve(foa_rx *rx, size_t n_samples, size_t n_frames);
  *                 after foa_rx_sync (or, for the call before the most recent one, after foa_rx_wait_previous), and the INPUTS of a call
  *                 must be complete when it is made and stay untouched until then.  0 = every call runs start to end on the handle's
  *                 stream.  (Waits for everything in flight before it switches.)
- *   "depth"       pipelined calls: how many calls' loops are in flight -- 0 (default) = by grid size: 2 (3 for BPSK-only captures: option "max_dbps" <= 36), or 4 for calls of up to 4608 frames,
- *                 whose forward pass leaves most SIMDs a single wave (1 000-frame batches decode 40-50 % faster in steady state); 2, 3, 4 =
- *                 fixed.  (the lanes share the process's hardware queues, see above)
+ *   "depth"       pipelined calls: how many calls' loops are in flight -- 0 (default) = by grid size: 2, or 3 for BPSK-only captures (option "max_dbps" <= 36) and for calls of up to 6144 frames,
+ *                 whose forward pass leaves SIMDs idle (calls of 1 000 frames take 0.24 ms instead of 0.30 in steady state) -- but 2 for a call
+ *                 behind a device pre-sync or an upload, which share the third lane's hardware queue; 2, 3, 4 = fixed.
  *   "max_dbps"    what the work sets of later calls (and foa_rx_reserve) are sized for: the data bits per OFDM symbol of the HIGHEST rate the
  *                 caller's frames carry, 24 (6 Mbps) .. 216 (54 Mbps, the default: any rate).  A call's per-step buffers -- 10.25 bytes per
  *                 trellis step, several sets in rotation -- hold n_samples / 80 x max_dbps steps, so a capture of 6 Mbps frames needs a

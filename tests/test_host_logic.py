@@ -34,3 +34,7 @@ def test_every_stream_has_the_default_priority(tmp_path):
 
 def test_a_host_decode_copies_its_inputs_behind_the_frames_being_built(tmp_path):
     assert "all checks passed" in build_and_run(tmp_path, "scratch_order")
+
+
+def test_a_handles_streams_sit_on_queues_of_their_own_whatever_the_host_made(tmp_path):
+    assert "all checks passed" in build_and_run(tmp_path, "stream_order")
