@@ -17,8 +17,7 @@ struct ShardDev {
     DevBuf<float> dev[foa::kStreamBufs];
     DevBuf<uint8_t> d_desc[foa::kStreamBufs];
     DevBuf<int64_t> d_ends[foa::kStreamBufs];
-    hipEvent_t in_done[foa::kStreamBufs] = {}, sel_done[foa::kStreamBufs] = {}, sync_done[foa::kStreamBufs] = {};
-    hipStream_t st_in = nullptr;
+    hipEvent_t sel_done[foa::kStreamBufs] = {}, sync_done[foa::kStreamBufs] = {};
     hipStream_t st_sel = nullptr;                    // the chain's own stream: a batch's look-ahead waits for that batch's pre-sync and nothing else -- on the
                                                      // side stream it would sit behind the pre-syncs of the device's NEXT batches, which are staged ahead
     DevBuf<StreamState> state;                       // the chain state as handed in, moved on by the look-ahead
@@ -55,13 +54,10 @@ struct ShardDev {
             rc = dev[i].ensure((size_t)(foa::kStreamCarry + B) * 2);
             if (!rc) rc = d_desc[i].ensure(desc_cap * sizeof(foa_frame_desc));
             if (!rc) rc = d_ends[i].ensure(desc_cap);
-            if (!rc && hipEventCreateWithFlags(&in_done[i], hipEventDisableTiming) != hipSuccess) rc = fail(FOA_E_HIP, "hipEventCreate failed");
             if (!rc && hipEventCreateWithFlags(&sel_done[i], hipEventDisableTiming) != hipSuccess) rc = fail(FOA_E_HIP, "hipEventCreate failed");
             if (!rc && hipEventCreateWithFlags(&sync_done[i], hipEventDisableTiming) != hipSuccess) rc = fail(FOA_E_HIP, "hipEventCreate failed");
         }
-        // (made behind the handle's six, these two share hardware queues with streams of it: rx_handle.hip, foa_rx_create)
         if (!rc && hipStreamCreateWithFlags(&st_sel, hipStreamNonBlocking) != hipSuccess) rc = fail(FOA_E_HIP, "hipStreamCreate failed");
-        if (!rc && hipStreamCreateWithFlags(&st_in, hipStreamNonBlocking) != hipSuccess) rc = fail(FOA_E_HIP, "hipStreamCreate failed");
         if (!rc && hipHostMalloc((void **)&sel, (size_t)foa::kStreamBufs * 8 * sizeof(int32_t), hipHostMallocDefault) != hipSuccess) rc = fail(FOA_E_NOMEM, "hipHostMalloc failed");
         if (!rc && hipHostMalloc((void **)&st_pin, (size_t)foa::kStreamBufs * 2 * sizeof(StreamState), hipHostMallocDefault) != hipSuccess) rc = fail(FOA_E_NOMEM, "hipHostMalloc failed");
         if (!rc) rc = sel_dev.ensure((size_t)foa::kStreamBufs * 8);
@@ -83,14 +79,12 @@ struct ShardDev {
         while (!flight.empty()) { foa::StreamReady r; if (collect(flight.front().handle, true, &r) <= 0) break; }
         for (int i = 0; i < foa::kStreamBufs; i++) {
             dev[i].release(); d_desc[i].release(); d_ends[i].release();
-            if (in_done[i]) (void)hipEventDestroy(in_done[i]);
             if (sel_done[i]) (void)hipEventDestroy(sel_done[i]);
             if (sync_done[i]) (void)hipEventDestroy(sync_done[i]);
-            in_done[i] = sel_done[i] = sync_done[i] = nullptr;
+            sel_done[i] = sync_done[i] = nullptr;
         }
-        if (st_in) (void)hipStreamDestroy(st_in);
         if (st_sel) (void)hipStreamDestroy(st_sel);
-        st_in = st_sel = nullptr;
+        st_sel = nullptr;
         if (sel) (void)hipHostFree(sel);
         if (st_pin) (void)hipHostFree(st_pin);
         sel = nullptr; st_pin = nullptr;
@@ -104,11 +98,12 @@ struct ShardDev {
         const int64_t C = foa::kStreamCarry;
         HIP_TRY(enter_device(rx->device));
         float *d = dev[k].p;
-        HIP_TRY(hipMemcpyAsync(d, carry, (size_t)C * 8, hipMemcpyHostToDevice, st_in));
-        if (n_new) HIP_TRY(hipMemcpyAsync(d + 2 * C, batch, (size_t)n_new * 8, hipMemcpyHostToDevice, st_in));
-        HIP_TRY(hipEventRecord(in_done[k], st_in));
+        // (on the pre-sync's stream: one of their own, made behind the handle's six, shares a hardware queue with lane 1 or 2 -- rx_handle.hip,
+        // foa_rx_create -- and an upload there waits for a forward pass: one device, 256 Ki-sample batches 0.52 -> 0.98 Gsample/s, 64 Ki 0.22 -> 0.27,
+        // 4 Mi within 6 % either way)
         hipStream_t st = side_stream(rx);
-        HIP_TRY(hipStreamWaitEvent(st, in_done[k], 0));
+        HIP_TRY(hipMemcpyAsync(d, carry, (size_t)C * 8, hipMemcpyHostToDevice, st));
+        if (n_new) HIP_TRY(hipMemcpyAsync(d + 2 * C, batch, (size_t)n_new * 8, hipMemcpyHostToDevice, st));
         n_buf[k] = C + n_new; start_abs[k] = start;
         int rc = sync_dev_issue(rx, d, (size_t)n_buf[k], (foa_frame_desc *)d_desc[k].p, d_ends[k].p, desc_cap, &ccap[k], start);
         if (rc) return rc;

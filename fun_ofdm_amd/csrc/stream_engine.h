@@ -132,7 +132,7 @@ struct StreamGpu {
     foa_rx *rx = nullptr;
     int64_t B = 0;                                   // batch_samples
     int n_bufs = 6;                                  // buffers in rotation (foa_stream_create)
-    bool copies_in_line = false;                     // small batches: upload and carry copy on the pre-sync's own stream (stage_impl)
+    bool copies_in_line = false;                     // upload and carry copy on the pre-sync's own stream (stage_impl, foa_stream_create)
     bool fill_by_kernel = false;                     // ... and done by one kernel that reads the page-locked staging memory itself
     int64_t L = foa::kStreamLongest, C = foa::kStreamCarry;      // longest frame the stream may hold (+ look-ahead) and the carry it implies (option "stream_longest")
     size_t slot_bytes = 4096;
@@ -327,8 +327,12 @@ int foa_stream_create(foa_rx *rx, size_t batch_samples, int narrow_threads, foa_
     // -- 4 .. 16 Ki samples at 20 Msample/s -- need more than six of them on their way at once; with six -- five staged or in flight -- the engine's capacity at 4 Ki
     // samples is 23 Msample/s, and a backlog, once there, drains at 3 while the caller waits for staging slots (profiles/r06_latency_stages.txt).  FOA_STREAM_BUFS overrides (A/B).
     g.n_bufs = batch_samples <= ((size_t)1 << 16) ? foa::kStreamBufs : 6;
-    g.copies_in_line = batch_samples <= ((size_t)1 << 16) && !getenv("FOA_STREAM_COPY_STREAM");
-    g.fill_by_kernel = g.copies_in_line && !getenv("FOA_STREAM_DMA_UPLOAD");
+    // (the upload: on the pre-sync's own stream for small batches, see stage_impl, and for those with two loops in flight, because a stream made
+    // behind the handle's six shares a hardware queue with lane 1 or 2 -- foa_rx_create -- and an upload there waits for a forward pass: 4 Mi-sample
+    // batches 3.95 -> 5.17 Gsample/s in calls of 64 Ki samples, 3.22 -> 3.63 in calls of 4 Ki; with four loops, 256 Ki-sample batches lose, 1.10 -> 0.85: profiles/stream_order.txt)
+    const bool small = batch_samples <= ((size_t)1 << 16), two_loops = batch_samples > ((size_t)1 << 20) || rx->max_depth < 4;
+    g.copies_in_line = (small || two_loops) && !getenv("FOA_STREAM_COPY_STREAM");
+    g.fill_by_kernel = small && g.copies_in_line && !getenv("FOA_STREAM_DMA_UPLOAD");
     if (const char *e = getenv("FOA_STREAM_BUFS")) { const int v = atoi(e); if (v >= 3 && v <= foa::kStreamBufs) g.n_bufs = v; }
     int rc = FOA_OK;
     for (int i = 0; i < g.n_bufs && !rc; i++) {
@@ -381,7 +385,7 @@ int foa_stream_create(foa_rx *rx, size_t batch_samples, int narrow_threads, foa_
     rx->finish_in_line = batch_samples >= 8192 && batch_samples <= ((size_t)1 << 16) && !getenv("FOA_STREAM_FINISH_STITCH");
     rx->timing = false;                              // (nobody reads per-kernel times of a stream's batches: seven runtime calls less per batch)
     rx->depth_saved = rx->depth;
-    rx->depth = (batch_samples <= ((size_t)1 << 20) && rx->max_depth >= 4) ? 4 : 2;
+    rx->depth = two_loops ? 2 : 4;
     if (const char *e = getenv("FOA_STREAM_DEPTH")) { const int v = atoi(e); if (v >= 2 && v <= 4) rx->depth = v; }
     // (and the submitter thread of such a stream polls instead of sleeping while batches keep coming: stream_core.h; FOA_STREAM_SPIN_US overrides, 0 = it sleeps)
     int spin_us = batch_samples <= ((size_t)1 << 16) ? 2000 : 0;
