@@ -1,4 +1,4 @@
-// foa_sim -- offline receiver over a raw I/Q file (SURVEY 8f #4; the shape of the reference's examples/test_sim.cpp
+// foa_sim -- offline receiver over a raw I/Q file (the shape of the reference's examples/test_sim.cpp
 // with the simulated channel replaced by a capture).
 //
 //   foa_sim <iq file> [--format fc32|fc64] [--chunk N] [--device D] [--async K] [--device-batch B [--narrow-threads T] [--devices D0,D1,..]]
@@ -77,7 +77,7 @@ int main(int argc, char **argv)
     // A caller that hands process_samples() megabyte-sized vectors at gigabytes per second must not have its allocator give every one of
     // them back to the kernel: glibc serves requests above its mmap threshold (128 KB until the first such block is freed, then whatever
     // that block's size was) with a mapping of their own, and freeing 3.5 GB of those costs 0.2-0.3 s of munmap -- page by page, under the
-    // process's mmap lock -- which is where calls of >= 65 536 samples spent their time in round 3 (0.64-0.70 Gsample/s against 4 with
+    // process's mmap lock -- which is where calls of >= 65 536 samples spent their time before (0.64-0.70 Gsample/s against 4 with
     // calls of 4096 samples, whose 64 KB vectors come from the heap).  A long-running receiver reaches the same state by itself (the
     // threshold adapts to the sizes it frees); --preload allocates every chunk before it frees the first, so it says so up front.
     mallopt(M_MMAP_THRESHOLD, 32 * 1024 * 1024);

@@ -13,7 +13,7 @@
 //   * soft bytes are scattered into the symbol's depunctured order in LDS ((carrier, bit) -> position table per
 //     rate), and leave in 8-byte stores, four trellis steps per lane and trip.
 // The kernel is persistent and keeps three groups of symbols in flight per wave (below: "the kernel"): 256 VGPRs, two waves per SIMD,
-// one beside the five waves of a forward pass when calls are pipelined (0.15 ms alone at config 2; HISTORY.md has the forms it replaced).
+// one beside the five waves of a forward pass when calls are pipelined (0.15 ms alone at config 2).
 #pragma once
 
 #include "device_math.h"
@@ -129,7 +129,7 @@ __device__ __forceinline__ void q4_emit(Q4Shared &sh, Q4Wave &ws, const cpx (&X)
 
 // ---- the kernel: persistent workgroups, three groups of symbols in flight per wave -----------------------------------------------------
 //
-// Rounds 1-5 launched one workgroup per 64 symbols.  Alone on the machine a wave of that kernel lived ~40 000 clocks for ~7 000 clocks
+// The form before launched one workgroup per 64 symbols.  Alone on the machine a wave of that kernel lived ~40 000 clocks for ~7 000 clocks
 // of its own issue: the tables went into LDS once per workgroup, and then one memory round trip waited for the next -- symbol -> frame,
 // frame record, descriptor, samples, four rounds of taps -- with three waves per SIMD to hide them behind.  It ran at 2.3 TB/s = 29 %
 // of HBM with the vector pipes a third busy, and it is what bounds the low rates (24 trellis steps per symbol instead of 216).

@@ -1,7 +1,7 @@
 // probe_kernels.h -- what does one wave64 instruction cost a SIMD on THIS part, now?  (foa_rx_probe_issue)
 //
 // bench.py's roofline prices the forward pass against the rate at which the machine can issue the instructions the pass is
-// made of.  That rate is measured live, in the run that reports it (VERDICT round 2: counters and clocks of another box do
+// made of.  That rate is measured live, in the run that reports it (counters and clocks of another box do
 // not belong in the line): 1024 SIMDs x W single-wave workgroups issue one instruction class from eight independent
 // chains for a fixed WINDOW of shader clocks (s_memtime ticks = shader cycles, MI355X_MICROARCH.md) and report how far
 // they got; the wall time of the launch (HIP events) gives the clock the part sustained meanwhile.

@@ -1,4 +1,4 @@
-// rx_sync.hip -- pre-sync (SURVEY 8f #1): frame_detector + timing_sync on the device over a resident stream (foa_rx_sync_dev*),
+// rx_sync.hip -- pre-sync: frame_detector + timing_sync on the device over a resident stream (foa_rx_sync_dev*),
 // and their streaming host restatement (foa_sync_*, sync_host.h).
 #include <algorithm>
 
@@ -44,7 +44,7 @@ int foa::sync_dev_issue(foa_rx *rx, const float *d_iq, size_t n_samples, foa_fra
     // (nothing else orders this stage behind the decode calls in flight, whose header and data-symbol kernels may still be reading the
     // descriptor buffers a caller reuses from round to round: wait for the front end of every one that reads what this stage is about to
     // write -- and of no other.  A caller that alternates two descriptor sets has the pre-sync of batch k + 1 running while batch k's front
-    // end still reads the other set: round 5 waited for the LATEST call's front end whatever it read, which put the pre-sync behind the
+    // end still reads the other set: an earlier form waited for the LATEST call's front end whatever it read, which put the pre-sync behind the
     // data-symbol kernel and the next front end behind the pre-sync -- one chain per step, 0.2 ms longer than the forward pass's)
     if (st != rx->stream) {
         const uint8_t *w0 = (const uint8_t *)d_descs, *w1 = w0 + cap * sizeof(foa_frame_desc), *e0 = (const uint8_t *)d_ends, *e1 = e0 + cap * sizeof(int64_t);
@@ -58,7 +58,7 @@ int foa::sync_dev_issue(foa_rx *rx, const float *d_iq, size_t n_samples, foa_fra
     // The flag kernel streams the whole capture through HBM, and so does the chain-back walk of the decode call two back, which is running
     // about now and sits on the loop that sets the step (forward pass k, walk k, front end k + 2 on one lane): side by side they share the
     // memory pipe and the walk -- the one somebody waits for -- takes longer.  Behind the walk the flags run under the second half of a
-    // forward pass, when nothing else wants HBM: BASELINE config 2 with the pre-sync in the loop 1.16 -> 1.08 ms per step
+    // forward pass, when nothing else wants HBM: 10 000 frames per call with the pre-sync in the loop 1.16 -> 1.08 ms per step
     // (profiles/r06_ab_presync_behind_walk.txt).  (The stream engines' batches are small and latency-bound: they do not wait.)
     if (behind_walk && st != rx->stream && rx->last_walk_done) HIP_TRY(hipStreamWaitEvent(st, rx->last_walk_done, 0));
     if ((rc = wait_after(rx, st))) return rc;                          // foa_rx_after: the caller's producers, on the device

@@ -1,4 +1,4 @@
-// rx_tx.hip -- the transmit side on the device: frame_builder::build_frame and the synthetic channel of SURVEY 8d,
+// rx_tx.hip -- the transmit side on the device: frame_builder::build_frame and the synthetic channel,
 // so that large synthetic workloads and loop-back tests live in HBM.
 #include "rx_handle.h"
 #include "tx_kernels.h"
@@ -60,7 +60,7 @@ int foa_tx_channel_dev(foa_rx *rx, const double *d_frames, size_t n_frames, size
     if (!d_frames || !d_iq) return fail(FOA_E_INVALID, "NULL device pointer");
     if (lead + frame_samples > pitch) return fail(FOA_E_INVALID, "lead + frame_samples exceeds the pitch");
     HIP_TRY(enter_device(rx->device));
-    // SURVEY 8d: sigma^2 per real component = P_ref / (2 10^(SNR/10)), P_ref = 0.0124
+    // sigma^2 per real component = P_ref / (2 10^(SNR/10)), P_ref = 0.0124
     const double sigma = std::sqrt(0.0124 / (2.0 * std::pow(10.0, snr_db / 10.0)));
     const int64_t total = (int64_t)n_frames * (int64_t)pitch;
     { int rc = wait_after(rx, rx->stream); if (rc) return rc; }

@@ -124,7 +124,7 @@ public:
             t.src = iq; t.is_double = sizeof(T) == sizeof(double); t.dst = be_->staging(slot) + 2 * fill_; t.n = take; t.slot = slot; t.owner = own; t.landed = nullptr;
             if (defer) {
                 // in slices of kPiece samples, each with its own reference to the buffer: a call of a million samples is then narrowed by
-                // every helper at once instead of by one (round 3: calls of >= 65536 samples ran at the rate of ONE helper), and the
+                // every helper at once instead of by one (before: calls of >= 65536 samples ran at the rate of ONE helper), and the
                 // caller still returns without touching a sample
                 for (size_t o = 0; o < take; o += kPiece) {
                     Task p = t;
@@ -189,7 +189,7 @@ private:
     // both sockets (EPYC 9575F, 220 M samples: 2.1 against 1.2-1.6 Gsample/s with four helpers).  So the engine's threads are
     // confined to the block of eight consecutive CPUs the creating thread runs on (one core complex where CPUs are numbered
     // core by core), within the process's own affinity mask.  FOA_STREAM_AFFINITY=0 leaves them to the scheduler.
-    // (Measured in round 3 and dropped: one core complex PER helper on the caller's NUMA node, from sysfs -- a task then takes a
+    // (Measured and dropped: one core complex PER helper on the caller's NUMA node, from sysfs -- a task then takes a
     // helper 7.2 us instead of 4.0, the buffers it releases belong to an allocator arena another complex owns, and the rate
     // falls from 2.2 to 1.7 Gsample/s; four helpers on one complex already move 100 GB/s.)
     void keep_threads_near_caller()
@@ -227,7 +227,7 @@ private:
     // A buffer of kBigOwner bytes or more is the allocator's own mapping (glibc: mmap from 128 KB), no arena is involved in freeing it, and
     // giving it back costs a munmap -- a quarter of a microsecond per page: 0.1-0.3 s for the 3.5 GB of a 220 M-sample capture handed over
     // in calls of 65536 samples or more.  Parked for the caller (below) that was the caller's time, and the reason why such calls ran at
-    // 0.64-0.70 Gsample/s in round 3 against 4 with calls of 4096; the helper that drops the last reference releases such a buffer itself.
+    // 0.64-0.70 Gsample/s before that against 4 with calls of 4096; the helper that drops the last reference releases such a buffer itself.
     static constexpr size_t kBigOwner = 128 * 1024;
     static constexpr size_t kPiece = 16384;          // samples per narrowing task of a large push
     struct Task { const void *src; bool is_double; float *dst; size_t n; int slot; Owner *owner; std::atomic<int64_t> *landed; };
@@ -335,7 +335,7 @@ private:
     }
     // Makes every written cell visible.  The caller does it every kPublish cells and wherever it is about to wait; the SUBMITTER does it
     // too, when cells have sat unpublished over two of its wake-ups while the caller made no call (a producer with a bounded pool of
-    // buffers waits for them to come back without calling anything: round 3's core then held on to its last < kPublish buffers for
+    // buffers waits for them to come back without calling anything: the core then held on to its last < kPublish buffers for
     // good).  Hence the claim: a range [pub_, tail_) belongs to whoever moves pub_ over it.
     void publish()
     {

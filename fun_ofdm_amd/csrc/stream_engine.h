@@ -1,4 +1,4 @@
-// stream_engine.h -- receiver_chain::process_samples() with EVERYTHING on the device (SURVEY 8f #1 + #3):
+// stream_engine.h -- receiver_chain::process_samples() with EVERYTHING on the device:
 // foa_stream_* of include/fun_ofdm_amd.h.  Host code only (rx_stream.hip); it drives the handle's streams, work sets and job slots.
 //
 // The reference runs frame_detector -> timing_sync -> fft_symbols -> ... -> frame_decoder inside every

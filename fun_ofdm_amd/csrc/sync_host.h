@@ -2,7 +2,7 @@
 //
 // The reference's two pre-sync blocks (frame_detector.cpp:41-93 with circular_accumulator.h:88-95, and
 // timing_sync.cpp:51-139) sit in front of the hot path inside receiver_chain::process_samples().
-// Until they run on the device (SURVEY 8f #1) this restatement supplies what the device path needs
+// Until they run on the device this restatement supplies what the device path needs
 // from them: where each LTS1 tag lands and which constant phasor timing_sync applies from where.
 // It never touches sample values (the rotation itself is applied in-kernel), so it only has to
 // reproduce the blocks' DECISIONS; it does that with the same operation order in fp64.
@@ -168,7 +168,7 @@ public:
                 d.rot_start = origin + (int64_t)x;
                 // cos and sin of ONE argument as the reference's build computes them: g++ -O3 turns the pair of calls in timing_sync.cpp:124
                 // into one sincos(), whose cosine is not always the bit pattern cos() returns (glibc; 1 ulp apart on 2 of 4 685 alignments of
-                // round 4's collision streams, where this file's separate calls -- clang keeps them separate -- were caught against the oracle,
+                // the collision streams, where this file's separate calls -- clang keeps them separate -- were caught against the oracle,
                 // which is compiled like the reference and equals its compiled timing_sync bit for bit on those streams)
                 phasor(phase_acc_, d.c, d.s);
                 phasor(prev, d.c_prev, d.s_prev);

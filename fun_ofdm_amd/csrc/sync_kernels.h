@@ -1,4 +1,4 @@
-// sync_kernels.h -- frame_detector + timing_sync on the device (SURVEY 8f #1).
+// sync_kernels.h -- frame_detector + timing_sync on the device.
 //
 // What the host restatement (sync_host.h) does sample by sample, restructured for a GPU:
 //   k_sync_flags     frame_detector.cpp:51-66: lag-16 autocorrelation / power over a 16-sample window, threshold 0.9.
@@ -210,7 +210,7 @@ __device__ __forceinline__ int block1024_exclusive_scan(int v, int32_t *part, in
 
 // exclusive scan of block counts; total -> out_total[0].  ONE WAVE: the stage runs under the forward pass of a decode call in flight, where a
 // 1024-thread block waits for sixteen free wave slots on one CU -- 240-320 us in the pipelined loop for 8 us of work (a kernel trace of
-// BASELINE config 2 with the pre-sync in the loop, profiles/r06_presync_timeline.txt; the decode call's own scan learnt this in round 3).
+// 10 000 frames per call with the pre-sync in the loop, profiles/r06_presync_timeline.txt; the decode call's own scan does the same).
 // 64 consecutive counts per turn (one coalesced load), four turns' loads in flight.
 __global__ __launch_bounds__(64) void k_sync_scan(const int32_t *__restrict__ cnt, int n_blocks, int32_t *__restrict__ off, int32_t *__restrict__ out_total)
 {

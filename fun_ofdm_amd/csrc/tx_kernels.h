@@ -1,4 +1,4 @@
-// tx_kernels.h -- frame_builder::build_frame on the device, plus the synthetic channel of SURVEY 8d.
+// tx_kernels.h -- frame_builder::build_frame on the device, plus the synthetic channel.
 //
 // The transmit side is not part of the receive hot path; it exists so that large synthetic workloads can be created
 // in HBM (80 000 frames are 2.25 GB of samples before padding) and so that device-resident loop-back tests are
@@ -128,7 +128,7 @@ __global__ __launch_bounds__(64) void k_tx_symbols(const uint8_t *__restrict__ s
     }
 }
 
-// ---- K3: the synthetic channel of SURVEY 8d: frames at a fixed pitch, per-frame carrier phase (and optional constant
+// ---- K3: the synthetic channel: frames at a fixed pitch, per-frame carrier phase (and optional constant
 // frequency offset), complex white Gaussian noise, rounding to complex<float>.  One thread per output sample; the random
 // numbers come from a counter hash, so the stream depends only on (seed, sample index). ----
 __device__ __forceinline__ uint64_t tx_mix64(uint64_t z)

@@ -26,7 +26,7 @@
 //   * The renormalisation test reads state 0 with one v_readfirstlane and decides on the scalar unit.
 //   * The same code with ONE frame per wave (template argument kPair = 1, the high halves idle and left alone) serves calls so small
 //     that every wave has a SIMD nearly to itself: a wave's own step latency and its renormalisation events are what such a call waits for.
-// What was measured on the way here and dropped is in HISTORY.md (patches and numbers under profiles/).
+// (What was measured on the way here and dropped: patches and numbers under profiles/.)
 #pragma once
 
 #include "device_math.h"
@@ -285,8 +285,8 @@ __device__ __forceinline__ uint32_t fwd3_group(uint32_t M, const uint4 *bml, con
 // The same six steps for a wave that has its SIMD to itself (one frame per wave): the increments of the group AFTER this one (entries
 // ENEXT .., -1: none) are read before the group's own steps, which use the ones the group before fetched (w) -- a lone wave has nobody to
 // hide an LDS round trip behind, and with the reads at the head of their own group it stood still for one every six steps (forward pass
-// of 16 .. 256 frames of 1 024 bytes at 54 Mbps: 0.445 -> 0.430 ms; with five waves to a SIMD the same change bought nothing, HISTORY.md).
-// (Tried on top of it and dropped, round 6: the six steps run WITHOUT the renormalisation test, state 0's largest metric of the group
+// of 16 .. 256 frames of 1 024 bytes at 54 Mbps: 0.445 -> 0.430 ms; with five waves to a SIMD the same change bought nothing).
+// (Tried on top of it and dropped: the six steps run WITHOUT the renormalisation test, state 0's largest metric of the group
 // tested once behind them and the group run again step by step when it fires -- a renormalisation is due every ~9 steps at 54 Mbps, so
 // half the groups run twice: 0.52 ms.)
 template <int E0, int J0, int ENEXT, typename Flush>

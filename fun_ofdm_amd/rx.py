@@ -215,7 +215,7 @@ class Receiver:
         return out
 
     def tx_channel(self, frames, pitch, lead, snr_db, seed, cfo_hz=0.0):
-        """Synthetic channel (SURVEY 8d) on the device: frames float64[n, S, 2] -> float32[n * pitch, 2] (CUDA tensors)."""
+        """Synthetic channel on the device: frames float64[n, S, 2] -> float32[n * pitch, 2] (CUDA tensors)."""
         import torch
         n, s, _ = frames.shape
         iq = torch.empty((n * pitch, 2), dtype=torch.float32, device=frames.device)

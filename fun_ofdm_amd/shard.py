@@ -1,7 +1,7 @@
 """Frame sharding across GPUs (one process per GPU, torch.distributed; backend "nccl" = RCCL over xGMI).
 
 Frames are independent, so the data path has no collective: global frame i lives on rank i mod G
-(BASELINE config 4) and is decoded there; the only exchange is one gather of the decoded PSDU slots to rank 0.
+and is decoded there; the only exchange is one gather of the decoded PSDU slots to rank 0.
 """
 import torch
 import torch.distributed as dist

@@ -3,7 +3,7 @@
 A vectorised restatement of the reference's transmit path -- frame_builder::build_frame
 (src/frame_builder.cpp:53-82) over ppdu::encode (src/ppdu.cpp:65-165), symbol_mapper::map
 (src/symbol_mapper.cpp:81-119) and fft::inverse (src/fft.cpp:68-96) -- so that thousands of distinct
-frames can be produced quickly.  It reproduces the reference's deviations from 802.11a (SURVEY A.0):
+frames can be produced quickly.  It reproduces the reference's deviations from 802.11a:
 generator masks {121,91} with the newest bit at the LSB, its puncturing patterns, the single 48-entry
 interleaver map, the byte-wise LSB scrambler, the 12-bit length field, and the literal preamble table.
 tests/test_synth.py checks it against the oracle's build_frame.
@@ -15,7 +15,7 @@ import numpy as np
 # src/rates.h:52-196: rate_field, cbps, dbps, bpsc, puncture (0: 1/2, 1: 2/3, 2: 3/4)
 RATES = ((0xD, 48, 24, 1, 0), (0xE, 48, 32, 1, 1), (0xF, 48, 36, 1, 2), (0x5, 96, 48, 2, 0), (0x6, 96, 64, 2, 1), (0x7, 96, 72, 2, 2),
          (0x9, 192, 96, 4, 0), (0xA, 192, 128, 4, 1), (0xB, 192, 144, 4, 2), (0x1, 288, 192, 6, 1), (0x3, 288, 216, 6, 2))
-P_REF = 0.0124          # nominal in-frame power used to set the AWGN level (SURVEY 8d)
+P_REF = 0.0124          # nominal in-frame power used to set the AWGN level
 
 _DATA_IDX = np.array([i for i in range(6, 59) if i not in (11, 25, 32, 39, 53)])
 _PILOT_IDX = np.array([11, 25, 39, 53])

@@ -16,7 +16,7 @@
  * is used from one thread at a time; each handle owns its HIP streams (below); there is NO CPU fallback -- a
  * call fails with FOA_E_NO_DEVICE when no gfx950 device/HIP runtime is usable.
  *
- * The reference-side binding a maintainer would add is shown in INTEGRATION.md.
+ * A host creates a handle, hands over samples and descriptors and collects PSDUs: examples/foa_sim.cpp is one.
  */
 #ifndef FUN_OFDM_AMD_H
 #define FUN_OFDM_AMD_H
@@ -119,7 +119,7 @@ int foa_rx_reserve(foa_rx *rx, size_t n_samples, size_t n_frames);
  *   "max_dbps"    what the work sets of later calls (and foa_rx_reserve) are sized for: the data bits per OFDM symbol of the HIGHEST rate the
  *                 caller's frames carry, 24 (6 Mbps) .. 216 (54 Mbps, the default: any rate).  A call's per-step buffers -- 10.25 bytes per
  *                 trellis step, several sets in rotation -- hold n_samples / 80 x max_dbps steps, so a capture of 6 Mbps frames needs a
- *                 ninth of the default, and a call can take nine times the frames (machine-filling calls at 6-18 Mbps: DESIGN.md 4).  A
+ *                 ninth of the default, and a call can take nine times the frames (machine-filling calls at 6-18 Mbps).  A
  *                 promise, checked on the device: a frame that does not fit in what is left of its call's work set is reported
  *                 FOA_ST_NO_SPACE, never decoded wrongly.  Results are otherwise identical for every value.
  *
@@ -213,7 +213,7 @@ void *foa_rx_stream(foa_rx *rx);
 /* The same with nothing left to wait for: foa_rx_submit_host copies the caller's buffers, queues the transfers and the decode
  * and returns a ticket; up to 8 calls may be in flight.  foa_rx_collect(ticket, wait, ...) returns 1 and fills psdu
  * (n_frames * slot_bytes) and results once that call is complete, 0 if it is not yet (only with wait = 0), < 0 on error.
- * Calls complete in the order they were submitted.  For a stream front end that must not stall on the GPU (SURVEY 8f #3):
+ * Calls complete in the order they were submitted.  For a stream front end that must not stall on the GPU:
  * H2D of batch k+1, compute of batch k and D2H of batch k-1 overlap on the library's streams. */
 int foa_rx_submit_host(foa_rx *rx, const float *iq, size_t n_samples, const foa_frame_desc *descs, const int64_t *ends, size_t n_frames,
                        size_t slot_bytes, uint64_t *ticket);
@@ -224,7 +224,7 @@ int foa_rx_collect(foa_rx *rx, uint64_t ticket, int wait, uint8_t *psdu, foa_fra
 
 /* ---- device-side ordering against the caller's own HIP streams -------------------------------------------------------------------------
  *
- * The plain entry points above keep SURVEY 8(b)'s contract in its simplest form: buffers handed to a call must be COMPLETE when the call
+ * The plain entry points above keep the contract of blocking calls in its simplest form: buffers handed to a call must be COMPLETE when the call
  * is made (and stay untouched until it has read them), and outputs are final after foa_rx_sync -- the host waits.  A caller whose samples
  * are produced on the device by a stream of its own (an SDR's DMA engine, a channel simulator, another library) orders the two on the
  * DEVICE instead: every `event` below is a hipEvent_t (passed as void * so that this header needs no HIP header), recorded or waited for
@@ -245,7 +245,7 @@ int foa_rx_collect(foa_rx *rx, uint64_t ticket, int wait, uint8_t *psdu, foa_fra
  *                                   a pipelined call at once (option "pipeline"), like foa_rx_sync does.
  *   foa_rx_decode_frames_dev_after / foa_rx_sync_dev_begin_after = foa_rx_after(rx, inputs_ready) + the call (inputs_ready may be NULL).
  *
- * A capture loop over two device buffers with no host synchronisation in it: INTEGRATION.md 2; tests/cpp/test_ordering.cpp runs one
+ * A capture loop over two device buffers with no host synchronisation in it: tests/cpp/test_ordering.cpp runs one
  * against the oracle.  The library's streams are non-blocking and know nothing of the caller's, so an un-ordered producer is overtaken
  * in both directions: order with these calls, or complete the buffers before the call. */
 int foa_rx_after(foa_rx *rx, void *event);
@@ -254,7 +254,7 @@ int foa_rx_record_done(foa_rx *rx, void *event);
 int foa_rx_decode_frames_dev_after(foa_rx *rx, void *inputs_ready, const float *d_iq, size_t n_samples, const foa_frame_desc *d_descs,
                                    const int64_t *d_ends, size_t n_frames, uint8_t *d_psdu, size_t slot_bytes, foa_frame_result *d_results);
 
-/* ---- pre-sync: on the host (streaming) and on the device (whole resident streams), SURVEY 8f #1 ---- */
+/* ---- pre-sync: on the host (streaming) and on the device (whole resident streams) ---- */
 
 /* Streaming frame_detector + timing_sync (src/frame_detector.cpp:41-93, src/timing_sync.cpp:51-139):
  * consumes the raw stream in chunks of any size and reports one descriptor per LTS1/LTS2 tag pair,
@@ -280,7 +280,7 @@ int foa_sync_set_call(foa_sync *s, int64_t call);
  * pointers, capacity cap) in stream order and returns the number of alignments in *n_found (synchronises).  The decisions
  * are the reference's up to floating-point ties: windowed sums are formed directly instead of by the reference's
  * ever-drifting running sums, so a threshold decision can differ when the normalised correlation is within ~1e-15 of
- * 0.9 (DESIGN.md 4) -- and the reference's running sums never quite forget a huge sample: after a glitch of >= ~1e10 times the
+ * 0.9 -- and the reference's running sums never quite forget a huge sample: after a glitch of >= ~1e10 times the
  * signal amplitude its frame_detector tags residue artefacts for the rest of the stream (circular_accumulator.h:88-95), which
  * this stage does not reproduce (it finds the real frames only; foa_sync_push_* reproduces the reference there as well;
  * tests/test_gpu_parity.py::test_device_sync_large_dynamic_range).  A NaN sample is taken in as the reference takes it -- the two
@@ -302,7 +302,7 @@ int foa_rx_sync_dev_end(foa_rx *rx, size_t *n_found);
 /* ... whose kernels start only after `inputs_ready` (a hipEvent_t of the caller's: "device-side ordering" above) */
 int foa_rx_sync_dev_begin_after(foa_rx *rx, void *inputs_ready, const float *d_iq, size_t n_samples, foa_frame_desc *d_descs, int64_t *d_ends, size_t cap);
 
-/* ---- process_samples() entirely on the device (SURVEY 8f #1 + #3): a stream engine over the calls above ------------
+/* ---- process_samples() entirely on the device: a stream engine over the calls above ------------
  *
  * What fun::receiver_chain::process_samples() does call by call (src/receiver_chain.cpp:106-126: frame_detector ->
  * timing_sync -> fft_symbols -> channel_est -> phase_tracker -> frame_decoder on a 4096-sample chunk, state carried from
@@ -357,7 +357,7 @@ int foa_stream_take(foa_stream *s, uint8_t *payloads, uint32_t *lengths);
  * submitted, [6] batches, [7] samples pushed */
 int foa_stream_stats(const foa_stream *s, uint64_t out[8]);
 
-/* ---- the same stream engine over SEVERAL devices (BASELINE config 4's frame sharding, behind the C ABI) -----------------------------
+/* ---- the same stream engine over SEVERAL devices (frames dealt out, behind the C ABI) -----------------------------
  *
  * foa_shard_* is foa_stream_* with a list of devices: batch k of the stream goes to device k mod n_devices -- upload, pre-sync,
  * decode and copy back on that device, through a receiver handle the shard creates for it -- so n_devices consecutive batches are in
@@ -367,7 +367,7 @@ int foa_stream_stats(const foa_stream *s, uint64_t out[8]);
  * left in force (timing_sync.cpp:113-125), 24 bytes the host hands from device to device in stream order (fun_ofdm_amd/csrc/shard_core.h; its ordering logic runs against
  * device doubles at 1, 2, 3 and 8 devices in tests/cpp/shard_core_test.cpp).  The payload list equals foa_stream_*'s and the reference
  * chain's (tests/test_gpu_stream.py runs it with the one device a test box has, listed once and twice).  A device may be listed more
- * than once (two handles on one device share it).  NOT measured on a multi-GPU node: none was available to the builder (DESIGN.md 7).
+ * than once (two handles on one device share it).  NOT measured on a multi-GPU node: none was available to the builder.
  * Threads, ownership of handed-over buffers and the meaning of every call are those of the foa_stream_* functions of the same name. */
 typedef struct foa_shard foa_shard;
 int foa_shard_create(const int *devices, int n_devices, size_t batch_samples, int narrow_threads, foa_shard **out);
@@ -414,7 +414,7 @@ int foa_decode_header_f64(foa_rx *rx, const double *carriers48, size_t n, foa_fr
 int foa_decode_data_f64(foa_rx *rx, const double *carriers, const uint64_t *carrier_off, size_t n_frames, foa_frame_result *results,
                         uint8_t *psdu, size_t slot_bytes);
 
-/* ---- transmit side on the device (SURVEY 8f #2): synthetic workloads and loop-back tests in HBM --------------------- */
+/* ---- transmit side on the device: synthetic workloads and loop-back tests in HBM --------------------- */
 
 /* frame_builder::build_frame (src/frame_builder.cpp:53-82: ppdu::encode src/ppdu.cpp:65-165, symbol_mapper::map
  * src/symbol_mapper.cpp:81-119, fft::inverse src/fft.cpp:68-96, preamble src/preamble.h:24) for n_frames payloads of the
@@ -423,7 +423,7 @@ int foa_decode_data_f64(foa_rx *rx, const double *carriers, const uint64_t *carr
  * Asynchronous on the handle's stream.  With n_frames = 0 only *frame_samples is computed. */
 int foa_tx_build_frames_dev(foa_rx *rx, const uint8_t *d_payloads, size_t payload_pitch, int length, int rate, size_t n_frames,
                             double *d_frames, size_t *frame_samples);
-/* The synthetic channel the benchmark workloads use (SURVEY 8d), not a reference component: frame i starts at sample
+/* The synthetic channel the benchmark workloads use, not a reference component: frame i starts at sample
  * i * pitch + lead of the output stream, gets a uniformly random carrier phase and, if cfo_hz > 0, a constant frequency
  * offset uniform in +-cfo_hz (20 Msample/s); complex white Gaussian noise with sigma^2 = 0.0124 / (2 10^(snr_db/10)) per
  * real component is added everywhere; the result is rounded to complex<float>.  Deterministic in (seed, sample index). */

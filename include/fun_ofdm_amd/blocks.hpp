@@ -310,7 +310,7 @@ inline int64_t pile_pos_(int64_t p) { return p; }
 inline size_t keep_pile_together(const std::deque<int64_t> &pending, size_t done) { return keep_pile_together(pending, done, pile_pos_); }
 
 // ---------------------------------------------------------------------------------------------------------------
-// rx_backend: fft_symbols + channel_est + phase_tracker + frame_decoder as ONE block (SURVEY 8b) for a chain that keeps the reference's
+// rx_backend: fft_symbols + channel_est + phase_tracker + frame_decoder as ONE block for a chain that keeps the reference's
 // own frame_detector and timing_sync threads: add_block(new fun_amd::rx_backend()) behind them instead of the four blocks
 // (src/receiver_chain.cpp:29-51).  It consumes the tagged, rotated samples timing_sync hands on (src/timing_sync.cpp:98-125: LTS1 /
 // LTS2 tags, every sample multiplied by the phasor in force) and makes ONE device call per work(): the fused kernels on those very
@@ -381,12 +381,12 @@ private:
 class receiver_chain {
 public:
     // async_batch_calls = 0: every call decodes what has completed and returns it (synchronous GPU call inside).
-    // async_batch_calls = k > 0: a stream front end that must keep up with the air (SURVEY 8f #3).  A lone frame takes the
+    // async_batch_calls = k > 0: a stream front end that must keep up with the air.  A lone frame takes the
     // GPU about a millisecond however short it is (its trellis is one serial chain), a batch of thousands hardly longer; so
     // every k-th call submits everything decodable as ONE asynchronous batch (foa_rx_submit_host: H2D, compute and D2H of
     // consecutive batches overlap) and every call hands out the payloads of the batches that have finished -- in stream
     // order, a few calls late, like the reference's five-call latency.  Same payloads as the synchronous mode.
-    // device_batch_samples = B > 0: the whole of process_samples() on the device (foa_stream_*, SURVEY 8f #1 + #3): samples are
+    // device_batch_samples = B > 0: the whole of process_samples() on the device (foa_stream_*): samples are
     // only narrowed to float on the host (narrow_threads helpers for large calls); every B samples one batch is uploaded,
     // pre-synchronised (frame_detector + timing_sync kernels), decoded and its payloads fetched, asynchronously; a call
     // returns the payloads of the batches that have finished, in stream order (latency: one batch; flush() at the end of a
@@ -397,7 +397,7 @@ public:
     {
         if (device_batch_ == 0) check(foa_sync_create(&sync_), "foa_sync_create");
     }
-    // SEVERAL devices (BASELINE config 4 behind process_samples): device mode with batch k of the stream on devices[k mod n] (foa_shard_*,
+    // SEVERAL devices (behind process_samples): device mode with batch k of the stream on devices[k mod n] (foa_shard_*,
     // include/fun_ofdm_amd.h) -- n consecutive batches in work at once, one receiver handle per entry of the list (a device may be listed
     // twice), payloads in stream order as ever.  Same payloads as every other mode.
     receiver_chain(const std::vector<int> &devices, size_t device_batch_samples, int narrow_threads = 0)
@@ -521,7 +521,7 @@ private:
     struct job { uint64_t ticket; size_t n_frames; bool final; std::vector<entry> sent; };     // sent: the alignments it decodes, stream-absolute
     static const int64_t kLongestFrame = 320 + 80 * 1369 + 160;       // samples: 4095 bytes at 6 Mbps, plus timing_sync's look-ahead
 
-    // the device consumes complex<float> (BASELINE north_star); the pre-sync decides on the doubles it was given
+    // the device consumes complex<float>; the pre-sync decides on the doubles it was given
     void append(const std::vector<std::complex<double> > &samples)
     {
         const size_t n = samples.size(), o = buf_.size();
@@ -707,7 +707,7 @@ private:
 };
 
 // ---------------------------------------------------------------------------------------------------------------
-// The caller of the boundary (SURVEY 8f #3): fun::receiver without the radio.
+// The caller of the boundary: fun::receiver without the radio.
 // ---------------------------------------------------------------------------------------------------------------
 // What usrp::get_samples(num_samples, buffer) (src/usrp.cpp:125-130) is to fun::receiver: fills `buffer` with the next
 // num_samples complex<double> samples.  Returning false ends the stream (a radio never does).
@@ -735,7 +735,7 @@ private:
     size_t pos_;
 };
 
-// Raw interleaved I/Q files (SURVEY 8f #4): "fc32" = complex<float> (GNU Radio / UHD rx_samples_to_file default),
+// Raw interleaved I/Q files: "fc32" = complex<float> (GNU Radio / UHD rx_samples_to_file default),
 // "fc64" = complex<double> (UHD's wire format for this reference, src/usrp.cpp:46).
 class file_source : public sample_source {
 public:

@@ -1,6 +1,6 @@
 /*
  * fun_ofdm_amd_diag.h -- diagnostics and measurement surface of libfun_ofdm_amd.so: kernel timings, intermediates of a decode call,
- * an issue-rate probe.  NOT part of the drop-in boundary (include/fun_ofdm_amd.h is what INTEGRATION.md binds, and all a host of the
+ * an issue-rate probe.  NOT part of the drop-in boundary (include/fun_ofdm_amd.h is what a host binds, and all a host of the
  * receive path needs): the tests, bench.py and the tools under tools/ use these to check parity of intermediates (FFT / equaliser
  * output within 1e-4, soft bytes bit for bit) and to price the kernels against their rooflines.  Same library, no stability promise:
  * entry points here may change with the kernels they look into.
