@@ -1011,7 +1011,7 @@ def extra_legs(args, rx, dev, iq, descs, ends, real, psdu_dev_path, res_dev_path
             rows.append(row)
             del d_iq
         legs["config3_rate_sweep"] = {"table": "small batch", "frames_per_rate": n, "payload_bytes": length, "snr_db": 25.0, "counted_samples": "in-frame", "rates": rows,
-                                      "reading": "%d frames per call = %d forward-pass waves on 1 024 SIMDs: a lone wave's latency sets the time, four calls' loops in flight "
+                                      "reading": "%d frames per call = %d forward-pass waves on 1 024 SIMDs: a lone wave's latency sets the time, three calls' loops in flight "
                                                  "(option depth); the machine-filling figures are in config3_machine_filling" % (n, n // 2)}
     except Exception as e:
         legs["config3_rate_sweep"] = {"error": str(e)[-300:]}

@@ -173,8 +173,8 @@ int foa_rx_create(foa_rx **out, int device)
         HIP_TRY(hipStreamCreateWithFlags(&rx->stream3, hipStreamNonBlocking));      // copies / pre-sync
         if (q && atoi(q) < 4) {                                          // (also set but empty = 1) fewer queues than lanes
             rx->max_depth = 2;
-            rx->notes += "GPU_MAX_HW_QUEUES is set below 4: the four lanes of small decode calls would share hardware queues, so such calls keep 2 loops in "
-                         "flight instead of 4; leave the variable unset (the runtime's default is 4). ";
+            rx->notes += "GPU_MAX_HW_QUEUES is set below 4: the lanes of small decode calls would share hardware queues, so such calls keep 2 loops in "
+                         "flight instead of 3, small batches of a stream 2 instead of 4; leave the variable unset (the runtime's default is 4). ";
         }
     }
     HIP_TRY(hipEventCreateWithFlags(&rx->in_ready, hipEventDisableTiming));
